@@ -59,6 +59,7 @@ extern "C" {
  * benchmark contract is quoted in bf16; both run on the same kernels. */
 #define MOE_DTYPE_BF16 0
 #define MOE_DTYPE_F16 1
+#define MOE_DTYPE_F32 2           /* only where an entry point says so */
 
 const char* moe_last_error(void);
 int moe_abi_version(void);
@@ -123,6 +124,42 @@ int moe_route_histogram_static(const void* topk_idx, int idx_is_int64, int64_t n
  */
 int moe_gather_rows(const void* src, const int32_t* perm, int div, int64_t n_rows, int64_t cols,
                     void* dst, const float* w_src, float* w_dst, void* stream);
+
+/* ---- tokens sorted by expert and back, with gradients ------------------------------
+ * No counterpart in the reference (its layer sorts on the host and has no gradient).
+ * Entry i = t*k + j is slot j of token t; ids[i] its expert.  An id outside [0,E) marks an
+ * entry without an expert (a padded token, an entry over an expert's capacity).
+ *
+ * moe_sort: stable sort of the n entries, those without an expert behind all others.
+ * counts int32 [E+1] and offsets int32 [E+2] (exclusive prefix) have one more group for
+ * them: offsets[E] is the number of rows that hold an entry, offsets[E+1] = n.
+ * perm[p] = entry at sorted row p, row_of[i] = row of entry i (inverse).
+ */
+size_t moe_sort_workspace(int64_t n, int E);
+int moe_sort(const void* ids, int idx_is_int64, int64_t n, int E, int32_t* counts, int32_t* offsets,
+             int32_t* perm, int32_t* row_of, void* ws, size_t ws_bytes, void* stream);
+
+/* dst[row_of[t*k+j], :] = src[t, :] for rows of row_bytes bytes of any type; zeros in the rows
+ * from *live (a device int32: offsets + E of moe_sort) on.  src_stride in bytes; dst has T*k
+ * packed rows.  Rows whose number is not in [0, T*k) are not followed.
+ */
+int moe_permute(const void* src, int64_t src_stride, int64_t row_bytes, const int32_t* row_of, const int32_t* live,
+                int64_t T, int k, void* dst, void* stream);
+
+/* out[t, :] = sum over j with row_of[t*k+j] in [0, *live) of weights[t*k+j] * rows[row_of[t*k+j], :];
+ * weights fp32 [T*k] or NULL (1 each).  rows of H elements of MOE_DTYPE_BF16 / F16 / F32, stride
+ * in elements; out packed, of the same type.  Sums in fp32 in slot order, one rounding.
+ */
+int moe_unpermute(const void* rows, int64_t rows_stride, const int32_t* row_of, const int32_t* live, const float* weights,
+                  int64_t T, int k, int64_t H, int dtype, void* out, void* stream);
+
+/* Gradient of moe_unpermute with weights: g_rows[row_of[i], :] = weights[i] * gy[t, :] (packed,
+ * T*k rows, zeros from *live on) and g_w[i] = <rows[row_of[i], :], gy[t, :]> (fp32, 0 for an
+ * entry without an expert).  Either may be NULL; rows is read for g_w only.
+ */
+int moe_unpermute_grad(const void* gy, int64_t gy_stride, const void* rows, int64_t rows_stride, const int32_t* row_of,
+                       const int32_t* live, const float* weights, int64_t T, int k, int64_t H, int dtype, void* g_rows,
+                       float* g_w, void* stream);
 
 /* ---- expert grouped GEMM (tcgen05 / TMEM / TMA) -----------------------------------
  * Replaces kernels/grouped_gemm_baseline.py:14-57, kernels/grouped_gemm_tilelang.py:119-214

@@ -24,6 +24,11 @@ SIGNATURES = {
     "moe_route_histogram": (_i32, [_vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp]),
     "moe_route_histogram_static": (_i32, [_vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "moe_gather_rows": (_i32, [_vp, _vp, _i32, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "moe_sort_workspace": (_sz, [_i64, _i32]),
+    "moe_sort": (_i32, [_vp, _i32, _i64, _i32, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "moe_permute": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _vp]),
+    "moe_unpermute": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _i32, _i64, _i32, _vp, _vp]),
+    "moe_unpermute_grad": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp]),
     "moe_grouped_gemm": (_i32, [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp]),
     "moe_grouped_gemm_gathered": (_i32, [_i32, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                          _i32, _i32, _i32, _i32, _vp, _vp]),

@@ -1,0 +1,351 @@
+// Tokens sorted by expert and back, with weights applied, and the gradients of both.
+//
+//   sort       the n = T*k entries (token t, slot j) by expert, stably, entries without an expert behind all others
+//   permute    rows[row_of[t,j], :] = x[t, :]                               zeros in the rows behind offsets[E]
+//   unpermute  y[t, :] = sum_j w[t,j] * rows[row_of[t,j], :]                entries without an expert add nothing
+//
+// The gradient of permute is unpermute without weights and the other way round; with weights unpermute has
+//   g_rows[row_of[t,j], :] = w[t,j] * gy[t, :]        g_w[t,j] = <rows[row_of[t,j], :], gy[t, :]>
+//
+// All of it is bound by memory.  Every kernel goes by tokens, not by sorted rows: a token's row is read once and written to
+// its k places (permute, gradient of unpermute), or its k rows are read and leave as one (unpermute), so nothing is read
+// twice and no sum needs an atomic; the order of every sum is fixed.
+#include "common.cuh"
+
+#include <cuda_fp16.h>
+
+namespace moe {
+namespace perm {
+
+template <int V> struct VecOf;
+template <> struct VecOf<16> { using type = uint4; };
+template <> struct VecOf<8> { using type = uint2; };
+template <> struct VecOf<4> { using type = uint32_t; };
+template <> struct VecOf<2> { using type = uint16_t; };
+template <> struct VecOf<1> { using type = uint8_t; };
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void from_f32(float x, float* o) { *o = x; }
+__device__ __forceinline__ void from_f32(float x, __half* o) { *o = __float2half_rn(x); }
+__device__ __forceinline__ void from_f32(float x, __nv_bfloat16* o) { *o = __float2bfloat16_rn(x); }
+
+// V bytes of elements of type T
+template <class T, int V>
+struct alignas(V) Pack {
+  static constexpr int N = V / (int)sizeof(T);
+  T e[N];
+};
+
+// rows that hold an entry: what lies behind them is read by nobody and holds zeros
+__device__ __forceinline__ int32_t live_rows(const int32_t* live, int64_t n) {
+  const int32_t v = *live;
+  return v < 0 ? 0 : ((int64_t)v > n ? (int32_t)n : v);
+}
+
+// One warp per token and segment of 32 * U vectors: the segment stays in registers while the k places are written.  U = 4
+// independent loads per lane, then k * U independent stores.
+template <int V>
+__global__ void __launch_bounds__(256)
+permute_kernel(const unsigned char* __restrict__ src, int64_t src_stride, const int32_t* __restrict__ row_of,
+               const int32_t* __restrict__ live, int64_t T, int k, int vecs, int segs, unsigned char* __restrict__ dst) {
+  using Vec = typename VecOf<V>::type;
+  constexpr int U = 4;
+  const int lane = threadIdx.x & 31;
+  const int64_t n = T * k, items = T * segs, nwarps = (int64_t)gridDim.x * 8;
+  const int32_t n_live = live_rows(live, n);
+  for (int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); item < items; item += nwarps) {
+    const int64_t t = item / segs;
+    const int v0 = (int)(item - t * segs) * (32 * U) + lane;
+    const Vec* s = reinterpret_cast<const Vec*>(src + t * src_stride);
+    Vec v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (v0 + 32 * u < vecs) v[u] = s[v0 + 32 * u];
+    for (int j0 = 0; j0 < k; j0 += 32) {
+      const int32_t mine = j0 + lane < k ? row_of[t * k + j0 + lane] : -1;
+      const int m = min(32, k - j0);
+      for (int j = 0; j < m; ++j) {
+        const int32_t r = __shfl_sync(0xFFFFFFFFu, mine, j);
+        if (r < 0 || r >= n) continue;
+        Vec* d = reinterpret_cast<Vec*>(dst) + (int64_t)r * vecs;
+        const bool has = r < n_live;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (v0 + 32 * u < vecs) d[v0 + 32 * u] = has ? v[u] : Vec{};
+      }
+    }
+  }
+}
+
+// One warp per token and segment of 32 * U vectors: the rows of eight slots are in flight before the first is added, and
+// they are added in slot order, in fp32, with one rounding at the end.
+template <class T, int V, int U>
+__global__ void __launch_bounds__(256)
+unpermute_kernel(const T* __restrict__ rows, int64_t rows_stride, const int32_t* __restrict__ row_of,
+                 const int32_t* __restrict__ live, const float* __restrict__ weights, int64_t tokens, int k, int vecs, int segs,
+                 T* __restrict__ out) {
+  using P = Pack<T, V>;
+  constexpr int J = 8 / U;
+  const int lane = threadIdx.x & 31;
+  const int64_t n = tokens * k, items = tokens * segs, nwarps = (int64_t)gridDim.x * 8;
+  const int32_t n_live = live_rows(live, n);
+  for (int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); item < items; item += nwarps) {
+    const int64_t t = item / segs;
+    const int v0 = (int)(item - t * segs) * (32 * U) + lane;
+    float acc[U][P::N];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < P::N; ++i) acc[u][i] = 0.f;
+    for (int j0 = 0; j0 < k; j0 += J) {
+      int32_t mine = -1;
+      float w = 1.f;
+      if (lane < J && j0 + lane < k) {
+        mine = row_of[t * k + j0 + lane];
+        if (weights) w = weights[t * k + j0 + lane];
+      }
+      if (mine >= n_live) mine = -1;
+      P p[J][U];
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int32_t r = __shfl_sync(0xFFFFFFFFu, mine, j);
+        const P* s = reinterpret_cast<const P*>(rows + (int64_t)r * rows_stride);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (r >= 0 && v0 + 32 * u < vecs) p[j][u] = s[v0 + 32 * u];
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int32_t r = __shfl_sync(0xFFFFFFFFu, mine, j);
+        const float wj = __shfl_sync(0xFFFFFFFFu, w, j);
+        if (r < 0) continue;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < P::N; ++i) acc[u][i] = weights ? fmaf(wj, to_f32(p[j][u].e[i]), acc[u][i]) : acc[u][i] + to_f32(p[j][u].e[i]);
+      }
+    }
+    P* d = reinterpret_cast<P*>(out) + t * vecs;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (v0 + 32 * u < vecs) {
+        P o;
+#pragma unroll
+        for (int i = 0; i < P::N; ++i) from_f32(acc[u][i], &o.e[i]);
+        d[v0 + 32 * u] = o;
+      }
+    }
+  }
+}
+
+// One CTA per token and run of up to eight slots: a piece of gy is read once, multiplied into the eight rows' places and
+// into eight sums over the width, which the CTA adds up at the end: lanes by shuffles, warps in their order.
+template <class T, int V>
+__global__ void __launch_bounds__(256)
+unpermute_grad_kernel(const T* __restrict__ gy, int64_t gy_stride, const T* __restrict__ rows, int64_t rows_stride,
+                      const int32_t* __restrict__ row_of, const int32_t* __restrict__ live, const float* __restrict__ weights,
+                      int64_t tokens, int k, int vecs, T* __restrict__ g_rows, float* __restrict__ g_w) {
+  using P = Pack<T, V>;
+  constexpr int J = 8;
+  __shared__ float part[8][J];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
+  const int runs = (k + J - 1) / J;
+  const int64_t n = tokens * k;
+  const int32_t n_live = live_rows(live, n);
+  for (int64_t item = blockIdx.x; item < tokens * runs; item += gridDim.x) {
+    const int64_t t = item / runs;
+    const int j0 = (int)(item - t * runs) * J, m = min(J, k - j0);
+    int32_t r[J];
+    float w[J], dot[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      r[j] = j < m ? row_of[t * k + j0 + j] : -1;
+      if (r[j] >= n) r[j] = -1;
+      w[j] = j < m ? weights[t * k + j0 + j] : 0.f;
+      dot[j] = 0.f;
+    }
+    const P* g = reinterpret_cast<const P*>(gy + t * gy_stride);
+    for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
+      const P gv = g[v];
+      P p[J];
+      if (g_w) {
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+          if (r[j] >= 0 && r[j] < n_live) p[j] = reinterpret_cast<const P*>(rows + (int64_t)r[j] * rows_stride)[v];
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        if (r[j] < 0) continue;
+        const bool has = r[j] < n_live;
+        if (g_w && has) {
+#pragma unroll
+          for (int i = 0; i < P::N; ++i) dot[j] = fmaf(to_f32(p[j].e[i]), to_f32(gv.e[i]), dot[j]);
+        }
+        if (g_rows) {
+          P o;
+#pragma unroll
+          for (int i = 0; i < P::N; ++i) from_f32(has ? w[j] * to_f32(gv.e[i]) : 0.f, &o.e[i]);
+          reinterpret_cast<P*>(g_rows)[(int64_t)r[j] * vecs + v] = o;
+        }
+      }
+    }
+    if (g_w) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) dot[j] = warp_sum(dot[j]);
+      if (lane == 0) {
+#pragma unroll
+        for (int j = 0; j < J; ++j) part[warp][j] = dot[j];
+      }
+      __syncthreads();
+      if (threadIdx.x < m) {
+        float s = 0.f;
+        for (int q = 0; q < nwarps; ++q) s += part[q][threadIdx.x];
+        g_w[t * k + j0 + threadIdx.x] = s;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+static int elem_bytes(int dtype) { return dtype == MOE_DTYPE_F32 ? 4 : 2; }
+
+// widest access that every row of these addresses and strides allows, in bytes (16, 8, 4 or narrower)
+static int vec_bytes(uintptr_t all) {
+  int v = 16;
+  while (v > 1 && (all & (uintptr_t)(v - 1))) v >>= 1;
+  return v;
+}
+
+static unsigned grid_for(int64_t items, int64_t per_cta, int64_t cap) {
+  int64_t b = ceil_div64(items, per_cta);
+  return (unsigned)(b < 1 ? 1 : (b > cap ? cap : b));
+}
+
+}  // namespace perm
+}  // namespace moe
+
+// ====================================================================================
+extern "C" size_t moe_sort_workspace(int64_t n, int E) { return moe_route_histogram_workspace(n, E + 1); }
+
+extern "C" int moe_sort(const void* ids, int idx_is_int64, int64_t n, int E, int32_t* counts, int32_t* offsets, int32_t* perm,
+                        int32_t* row_of, void* ws, size_t ws_bytes, void* stream) {
+  using namespace moe;
+  if (E < 1) return fail(MOE_ERR_ARG, "sort: bad expert count %d", E);
+  if (n > 0 && (!perm || !row_of)) return fail(MOE_ERR_ARG, "sort: null perm/row_of");
+  return route_histogram_ex(ids, idx_is_int64, n, E + 1, nullptr, counts, offsets, perm, row_of, ws, ws_bytes, nullptr, stream,
+                            ROUTE_KEEP_ALL, false);
+}
+
+extern "C" int moe_permute(const void* src, int64_t src_stride, int64_t row_bytes, const int32_t* row_of, const int32_t* live,
+                           int64_t T, int k, void* dst, void* stream) {
+  using namespace moe;
+  using namespace moe::perm;
+  if (T < 0 || k < 1 || row_bytes < 1 || src_stride < 0) return fail(MOE_ERR_ARG, "permute: bad shape T=%lld k=%d row bytes=%lld stride=%lld", (long long)T, k, (long long)row_bytes, (long long)src_stride);
+  if (T == 0) return MOE_OK;
+  if (!src || !row_of || !live || !dst) return fail(MOE_ERR_ARG, "permute: null pointer");
+  if (T * k > 0x7FFFFFFFll || row_bytes > 0x7FFFFFFFll) return fail(MOE_ERR_UNSUPPORTED, "permute: too many rows or too wide ones");
+  DeviceInfo dev;
+  int rc = current_device_info(&dev);
+  if (rc) return rc;
+  const int V = vec_bytes(reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst) | (uintptr_t)src_stride | (uintptr_t)row_bytes);
+  const int vecs = (int)(row_bytes / V), segs = (vecs + 127) / 128;
+  const unsigned grid = grid_for(T * segs, 8, (int64_t)dev.sm_count * 8);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const unsigned char* s = reinterpret_cast<const unsigned char*>(src);
+  unsigned char* d = reinterpret_cast<unsigned char*>(dst);
+#define MOE_PERMUTE(V_) permute_kernel<V_><<<grid, 256, 0, st>>>(s, src_stride, row_of, live, T, k, vecs, segs, d)
+  switch (V) {
+    case 16: MOE_PERMUTE(16); break;
+    case 8: MOE_PERMUTE(8); break;
+    case 4: MOE_PERMUTE(4); break;
+    case 2: MOE_PERMUTE(2); break;
+    default: MOE_PERMUTE(1); break;
+  }
+#undef MOE_PERMUTE
+  MOE_CHECK_LAUNCH("permute_kernel");
+  return MOE_OK;
+}
+
+template <class T, int V>
+static void launch_unpermute(const void* rows, int64_t stride, const int32_t* row_of, const int32_t* live, const float* w, int64_t tokens,
+                             int k, int64_t H, void* out, int sms, cudaStream_t st) {
+  using namespace moe::perm;
+  const int vecs = (int)(H * sizeof(T) / V);
+  constexpr int U = V == 16 ? 1 : 4;       // narrow vectors: more of them per lane
+  const int segs = (vecs + 32 * U - 1) / (32 * U);
+  unpermute_kernel<T, V, U><<<grid_for(tokens * segs, 8, (int64_t)sms * 8), 256, 0, st>>>(
+      reinterpret_cast<const T*>(rows), stride, row_of, live, w, tokens, k, vecs, segs, reinterpret_cast<T*>(out));
+}
+
+extern "C" int moe_unpermute(const void* rows, int64_t rows_stride, const int32_t* row_of, const int32_t* live, const float* weights,
+                             int64_t T, int k, int64_t H, int dtype, void* out, void* stream) {
+  using namespace moe;
+  using namespace moe::perm;
+  if (dtype < 0 || dtype > MOE_DTYPE_F32) return fail(MOE_ERR_ARG, "unpermute: unknown dtype %d", dtype);
+  if (T < 0 || k < 1 || H < 1 || rows_stride < 0) return fail(MOE_ERR_ARG, "unpermute: bad shape T=%lld k=%d H=%lld", (long long)T, k, (long long)H);
+  if (T == 0) return MOE_OK;
+  if (!rows || !row_of || !live || !out) return fail(MOE_ERR_ARG, "unpermute: null pointer");
+  if (T * k > 0x7FFFFFFFll || H > 0x1FFFFFFFll) return fail(MOE_ERR_UNSUPPORTED, "unpermute: too many rows or too wide ones");
+  DeviceInfo dev;
+  int rc = current_device_info(&dev);
+  if (rc) return rc;
+  const int w = elem_bytes(dtype);
+  const int V = vec_bytes(reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(out) | (uintptr_t)(rows_stride * w) | (uintptr_t)(H * w));
+  if (V < w) return fail(MOE_ERR_ARG, "unpermute: rows are not aligned to their element type");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+#define MOE_UNPERMUTE(T_, V_) launch_unpermute<T_, V_>(rows, rows_stride, row_of, live, weights, T, k, H, out, dev.sm_count, st)
+#define MOE_UNPERMUTE16(T_) (V == 16 ? MOE_UNPERMUTE(T_, 16) : V == 8 ? MOE_UNPERMUTE(T_, 8) : V == 4 ? MOE_UNPERMUTE(T_, 4) : MOE_UNPERMUTE(T_, 2))
+  if (dtype == MOE_DTYPE_F32) V == 16 ? MOE_UNPERMUTE(float, 16) : V == 8 ? MOE_UNPERMUTE(float, 8) : MOE_UNPERMUTE(float, 4);
+  else if (dtype == MOE_DTYPE_F16) MOE_UNPERMUTE16(__half);
+  else MOE_UNPERMUTE16(__nv_bfloat16);
+#undef MOE_UNPERMUTE16
+#undef MOE_UNPERMUTE
+  MOE_CHECK_LAUNCH("unpermute_kernel");
+  return MOE_OK;
+}
+
+template <class T, int V>
+static void launch_unpermute_grad(const void* gy, int64_t gy_stride, const void* rows, int64_t rows_stride, const int32_t* row_of,
+                                  const int32_t* live, const float* w, int64_t tokens, int k, int64_t H, void* g_rows, float* g_w,
+                                  int sms, cudaStream_t st) {
+  using namespace moe::perm;
+  const int vecs = (int)(H * sizeof(T) / V);
+  const unsigned threads = vecs >= 256 ? 256u : (unsigned)((vecs + 31) / 32 * 32);
+  const int64_t items = tokens * ((k + 7) / 8);
+  unpermute_grad_kernel<T, V><<<grid_for(items, 1, (int64_t)sms * 8), threads, 0, st>>>(
+      reinterpret_cast<const T*>(gy), gy_stride, reinterpret_cast<const T*>(rows), rows_stride, row_of, live, w, tokens, k, vecs,
+      reinterpret_cast<T*>(g_rows), g_w);
+}
+
+extern "C" int moe_unpermute_grad(const void* gy, int64_t gy_stride, const void* rows, int64_t rows_stride, const int32_t* row_of,
+                                  const int32_t* live, const float* weights, int64_t T, int k, int64_t H, int dtype, void* g_rows,
+                                  float* g_w, void* stream) {
+  using namespace moe;
+  using namespace moe::perm;
+  if (dtype < 0 || dtype > MOE_DTYPE_F32) return fail(MOE_ERR_ARG, "unpermute_grad: unknown dtype %d", dtype);
+  if (T < 0 || k < 1 || H < 1 || gy_stride < 0 || rows_stride < 0) return fail(MOE_ERR_ARG, "unpermute_grad: bad shape T=%lld k=%d H=%lld", (long long)T, k, (long long)H);
+  if (T == 0 || (!g_rows && !g_w)) return MOE_OK;
+  if (!gy || !row_of || !live || !weights || (g_w && !rows)) return fail(MOE_ERR_ARG, "unpermute_grad: null pointer");
+  if (T * k > 0x7FFFFFFFll || H > 0x1FFFFFFFll) return fail(MOE_ERR_UNSUPPORTED, "unpermute_grad: too many rows or too wide ones");
+  DeviceInfo dev;
+  int rc = current_device_info(&dev);
+  if (rc) return rc;
+  const int w = elem_bytes(dtype);
+  uintptr_t all = reinterpret_cast<uintptr_t>(gy) | (uintptr_t)(gy_stride * w) | (uintptr_t)(H * w) | reinterpret_cast<uintptr_t>(g_rows);
+  if (g_w) all |= reinterpret_cast<uintptr_t>(rows) | (uintptr_t)(rows_stride * w);
+  const int V = vec_bytes(all);
+  if (V < w) return fail(MOE_ERR_ARG, "unpermute_grad: rows are not aligned to their element type");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+#define MOE_UNPERMUTE(T_, V_) \
+  launch_unpermute_grad<T_, V_>(gy, gy_stride, rows, rows_stride, row_of, live, weights, T, k, H, g_rows, g_w, dev.sm_count, st)
+#define MOE_UNPERMUTE16(T_) (V == 16 ? MOE_UNPERMUTE(T_, 16) : V == 8 ? MOE_UNPERMUTE(T_, 8) : V == 4 ? MOE_UNPERMUTE(T_, 4) : MOE_UNPERMUTE(T_, 2))
+  if (dtype == MOE_DTYPE_F32) V == 16 ? MOE_UNPERMUTE(float, 16) : V == 8 ? MOE_UNPERMUTE(float, 8) : MOE_UNPERMUTE(float, 4);
+  else if (dtype == MOE_DTYPE_F16) MOE_UNPERMUTE16(__half);
+  else MOE_UNPERMUTE16(__nv_bfloat16);
+#undef MOE_UNPERMUTE16
+#undef MOE_UNPERMUTE
+  MOE_CHECK_LAUNCH("unpermute_grad_kernel");
+  return MOE_OK;
+}

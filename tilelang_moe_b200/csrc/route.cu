@@ -37,6 +37,7 @@ constexpr int RWPB = 8;            // warps per CTA in the count / scatter kerne
 // destination-major numbering used by expert parallelism.  Out-of-range ids come back as -1.
 // With kx > 0 the list is virtual: every run of kx stored ids (one token's routed experts) is followed by one entry
 // that is not stored anywhere and names expert E - 1, the shared expert riding along as one more group.
+// With kx = ROUTE_KEEP_ALL group E - 1 takes the entries whose id names none of the others.
 __device__ __forceinline__ int load_id(const void* ids, int is64, int64_t i, const int32_t* id_map, int E, int kx = 0) {
   if (kx > 0) {
     const int64_t t = i / (kx + 1);
@@ -45,6 +46,8 @@ __device__ __forceinline__ int load_id(const void* ids, int is64, int64_t i, con
     i = t * kx + sl;
     E -= 1;                          // stored ids name the routed experts only
   }
+  const bool keep_all = kx == ROUTE_KEEP_ALL;
+  if (keep_all) E -= 1;
   int e;
   if (is64) {
     const long long v = reinterpret_cast<const long long*>(ids)[i];
@@ -52,7 +55,7 @@ __device__ __forceinline__ int load_id(const void* ids, int is64, int64_t i, con
   } else {
     e = reinterpret_cast<const int*>(ids)[i];
   }
-  if (e < 0 || e >= E) return -1;
+  if (e < 0 || e >= E) return keep_all ? E : -1;
   return id_map ? id_map[e] : e;
 }
 

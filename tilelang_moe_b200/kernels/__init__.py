@@ -27,10 +27,13 @@ import torch
 
 from .. import layer as _layer
 from .. import ops as _ops
+from ..permute import MoESort, moe_permute, moe_sort, moe_unpermute
 
 __all__ = [
     "topk_softmax", "topk_softmax_best", "grouped_gemm", "grouped_gemm_best", "fusedmoe_tilelang", "fusedmoe",
     "FusedMoETileLang", "FusedMoE", "generate_fusedmoe_inputs", "route_histogram", "mhc_pre", "mhc_post",
+    # operators the reference does not have: tokens sorted by expert and back, with gradients
+    "MoESort", "moe_sort", "moe_permute", "moe_unpermute",
     # the reference's other public names (its strategy variants and its PyTorch baselines): the same operator each
     "topk_softmax_fused", "topk_softmax_selection", "topk_softmax_sonic", "topk_softmax_bitonic",
     "topk_softmax_separate", "topk_softmax_separate_compiled", "topk_softmax_tilelang_separate", "topk_radix_tilelang",

@@ -1,0 +1,189 @@
+"""Tokens sorted by expert and back, differentiable.
+
+    sort = moe_sort(ids, n_experts)                  tables of T tokens with k entries each, no host synchronisation
+    rows = moe_permute(x, sort)                      [T*k, H]: a copy of its token's row for every entry, by expert
+    y    = moe_unpermute(rows_out, sort, weights)    [T, H]: the k rows of a token, weighed and added up
+
+Rows sort.offsets[e] .. sort.offsets[e+1] - 1 belong to expert e.  An id outside [0, n_experts) marks an entry without an
+expert (a padded token, an entry over an expert's capacity): its row lies behind offsets[n_experts], holds zeros, and adds
+nothing; its gradients are zero.  Results and gradients are computed without atomics, in a fixed order.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import _lib, ops
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # MOE_DTYPE_* of include/moe_b200.h
+
+
+@dataclass(frozen=True)
+class MoESort:
+    """Tables of one routing: contiguous int32 tensors on one device, usable by any number of permutes and unpermutes."""
+    offsets: torch.Tensor    # [E + 1]: first row of every expert; offsets[E] rows hold an entry
+    perm: torch.Tensor       # [T * k]: entry t * k + j at each sorted row
+    row_of: torch.Tensor     # [T * k]: sorted row of each entry
+    k: int                   # entries per token
+
+    def __post_init__(self):
+        for name, t, least in (("offsets", self.offsets, 2), ("perm", self.perm, 0), ("row_of", self.row_of, 0)):
+            if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() < least:
+                raise ValueError(f"{name} must be a contiguous int32 vector")
+        if self.k < 1 or self.row_of.numel() % self.k or self.perm.numel() != self.row_of.numel():
+            raise ValueError(f"perm and row_of must have {self.k} entries for each token")
+        if not (self.offsets.device == self.perm.device == self.row_of.device):
+            raise ValueError("the tables of a sort must be on one device")
+
+    @property
+    def n_experts(self) -> int:
+        return self.offsets.numel() - 1
+
+    @property
+    def tokens(self) -> int:
+        return self.row_of.numel() // self.k
+
+
+def moe_sort(topk_ids: torch.Tensor, n_experts: int) -> MoESort:
+    """Stable sort of the entries of topk_ids [T, k] (or [T]; int32 or int64) by expert."""
+    ops._need_cuda(topk_ids)
+    if topk_ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError("expert ids must be int64 or int32")
+    if topk_ids.dim() not in (1, 2) or (topk_ids.dim() == 2 and topk_ids.shape[1] < 1):
+        raise ValueError("expert ids must be [T] or [T, k]")
+    if n_experts < 1:
+        raise ValueError(f"n_experts={n_experts} must be positive")
+    ids = topk_ids.contiguous()
+    n, dev = ids.numel(), ids.device
+    lib = _lib.load()
+    # one allocation: counts [E + 1], offsets [E + 2], perm [n], row_of [n]
+    buf = torch.empty(2 * n_experts + 3 + 2 * n, dtype=torch.int32, device=dev)
+    at = n_experts + 1
+    offsets, perm, row_of = buf[at:at + n_experts + 1], buf[at + n_experts + 2:at + n_experts + 2 + n], buf[at + n_experts + 2 + n:]
+    need = lib.moe_sort_workspace(n, n_experts)
+    ws = torch.empty(max(need, 4), dtype=torch.uint8, device=dev)
+    with ops._on(dev):
+        rc = lib.moe_sort(ops._ptr(ids), int(ids.dtype == torch.int64), n, n_experts, ops._ptr(buf), ops._ptr(offsets),
+                          ops._ptr(perm), ops._ptr(row_of), ops._ptr(ws), need, ops._stream())
+    _lib.check(rc, "moe_sort")
+    ops._after(dev)
+    return MoESort(offsets, perm, row_of, ids.shape[1] if ids.dim() == 2 else 1)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t with packed rows at any non-negative stride."""
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+def _stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _permute(x: torch.Tensor, sort: MoESort) -> torch.Tensor:
+    x = _rows(x)
+    T, H = x.shape
+    w = x.element_size()
+    out = torch.empty(T * sort.k, H, dtype=x.dtype, device=x.device)
+    with ops._on(x.device):
+        rc = _lib.load().moe_permute(ops._ptr(x), _stride(x) * w, H * w, ops._ptr(sort.row_of), ops._ptr(sort.offsets) + 4 * sort.n_experts,
+                                     T, sort.k, ops._ptr(out), ops._stream())
+    _lib.check(rc, "moe_permute")
+    ops._after(x.device)
+    return out
+
+
+def _unpermute(rows: torch.Tensor, sort: MoESort, weights: Optional[torch.Tensor]) -> torch.Tensor:
+    rows = _rows(rows)
+    T, H = sort.tokens, rows.shape[1]
+    out = torch.empty(T, H, dtype=rows.dtype, device=rows.device)
+    with ops._on(rows.device):
+        rc = _lib.load().moe_unpermute(ops._ptr(rows), _stride(rows), ops._ptr(sort.row_of), ops._ptr(sort.offsets) + 4 * sort.n_experts,
+                                       ops._ptr(weights), T, sort.k, H, _DTYPES[rows.dtype], ops._ptr(out), ops._stream())
+    _lib.check(rc, "moe_unpermute")
+    ops._after(rows.device)
+    return out
+
+
+def _unpermute_grad(gy: torch.Tensor, rows: Optional[torch.Tensor], sort: MoESort, weights: torch.Tensor, want_rows: bool,
+                    want_weights: bool):
+    gy = _rows(gy)
+    T, H = gy.shape
+    g_rows = torch.empty(T * sort.k, H, dtype=gy.dtype, device=gy.device) if want_rows else None
+    g_w = torch.empty(T, sort.k, dtype=torch.float32, device=gy.device) if want_weights else None
+    with ops._on(gy.device):
+        rc = _lib.load().moe_unpermute_grad(ops._ptr(gy), _stride(gy), ops._ptr(rows), 0 if rows is None else _stride(rows),
+                                            ops._ptr(sort.row_of), ops._ptr(sort.offsets) + 4 * sort.n_experts, ops._ptr(weights), T,
+                                            sort.k, H, _DTYPES[gy.dtype], ops._ptr(g_rows), ops._ptr(g_w), ops._stream())
+    _lib.check(rc, "moe_unpermute_grad")
+    ops._after(gy.device)
+    return g_rows, g_w
+
+
+class _Permute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, sort):
+        ctx.sort = sort
+        return _permute(x, sort)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        return _unpermute(g, ctx.sort, None), None
+
+
+class _Unpermute(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, weights, sort):
+        ctx.sort = sort
+        rows = _rows(rows)
+        # the rows are only kept where the weights' gradient needs them
+        ctx.save_for_backward(rows if weights is not None and ctx.needs_input_grad[1] else None, weights)
+        return _unpermute(rows, sort, weights)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        rows, weights = ctx.saved_tensors
+        if weights is None:
+            return _permute(gy, ctx.sort), None, None
+        return (*_unpermute_grad(gy, rows, ctx.sort, weights, ctx.needs_input_grad[0], ctx.needs_input_grad[1]), None)
+
+
+def _same_device(sort: MoESort, t: torch.Tensor, what: str) -> None:
+    if t.device != sort.row_of.device:
+        raise ValueError(f"{what} is on {t.device}, the sort's tables on {sort.row_of.device}")
+
+
+def moe_permute(x: torch.Tensor, sort: MoESort) -> torch.Tensor:
+    """Rows of x [T, H] at their entries' places: [T*k, H] of x's type.  Any element type; floating types of 16 and 32 bits
+    have a gradient, others (8-bit values beside their scales, say) are copied."""
+    ops._need_cuda(x)
+    if x.dim() != 2 or x.shape[1] < 1 or x.shape[0] != sort.tokens:
+        raise ValueError(f"x must be [{sort.tokens}, H], one row for each token of the sort")
+    _same_device(sort, x, "x")
+    if x.requires_grad and torch.is_grad_enabled():
+        if x.dtype not in _DTYPES:
+            raise ValueError("the gradient of moe_permute is computed in bfloat16, float16 or float32")
+        return _Permute.apply(x, sort)
+    return _permute(x, sort)
+
+
+def moe_unpermute(rows: torch.Tensor, sort: MoESort, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y[t] = sum over the entries of token t of weights[t, j] * its row: [T, H] of the rows' type (bfloat16, float16 or
+    float32), summed in fp32 in slot order and rounded once.  weights: float32 [T, k]; 1 where not given."""
+    ops._need_cuda(rows, weights)
+    if rows.dtype not in _DTYPES:
+        raise ValueError("rows must be bfloat16, float16 or float32")
+    if rows.dim() != 2 or rows.shape[1] < 1 or rows.shape[0] != sort.tokens * sort.k:
+        raise ValueError(f"rows must be [{sort.tokens * sort.k}, H], one for each entry of the sort")
+    _same_device(sort, rows, "rows")
+    if weights is not None:
+        if weights.dtype != torch.float32 or tuple(weights.shape) != (sort.tokens, sort.k):
+            raise ValueError(f"routing weights must be float32 [{sort.tokens}, {sort.k}]")
+        _same_device(sort, weights, "weights")
+        weights = weights.contiguous()
+    if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
+        return _Unpermute.apply(rows, weights, sort)
+    return _unpermute(rows, sort, weights)
