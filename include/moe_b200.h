@@ -161,6 +161,37 @@ int moe_unpermute_grad(const void* gy, int64_t gy_stride, const void* rows, int6
                        const int32_t* live, const float* weights, int64_t T, int k, int64_t H, int dtype, void* g_rows,
                        float* g_w, void* stream);
 
+/* ---- 8-bit operands ----------------------------------------------------------------
+ * No counterpart in the reference.  q e4m3, scale fp32; for a group of 128 elements of a row
+ * (the last of a row may be shorter): top = max(max |x|, 2^-100), scale = top / 448,
+ * q = e4m3(x * (448 / top)), to nearest even.  NaN and infinity: NaN in their places at least.
+ * dtype: MOE_DTYPE_BF16 / F16 / F32 of the input; strides in elements; q and scale packed.
+ *   rows     x [rows, K]            -> q [rows, K], scale [rows, ceil(K/128)]
+ *   silu_mul gate, up [rows, I]     -> the same of gate * sigmoid(gate) * up, computed in fp32
+ *   blocks   w [E, rows, K] packed  -> q, scale [E, ceil(rows/128), ceil(K/128)]: groups of 128 x 128
+ */
+int moe_fp8_quantize_rows(const void* x, int64_t x_stride, int64_t rows, int K, int dtype, void* q, float* scale,
+                          void* stream);
+int moe_fp8_silu_mul(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, int64_t rows, int I,
+                     int dtype, void* q, float* scale, void* stream);
+int moe_fp8_quantize_blocks(const void* w, int64_t E, int64_t rows, int K, int dtype, void* q, float* scale,
+                            void* stream);
+
+/* ---- 8-bit GEMM with a scale for each block of 128 (tcgen05 / TMEM / TMA) --------------
+ * Y[r, n] = sum_kb a_scale[r, kb] * b_scale[e, n/128, kb] * sum_{k in block kb} A[r, k] * B[e, n, k]
+ *   A        e4m3 [rows, K], row stride lda bytes (a multiple of 16); K a multiple of 16
+ *   a_scale  fp32, element (r, kb) at r * as_row + kb * as_k
+ *   B        e4m3 [E, N, K] packed;  b_scale fp32 [E, ceil(N/128), ceil(K/128)] packed
+ *   offsets  int32 [E+1] on the device: group e owns rows offsets[e] .. offsets[e+1]-1.  NULL
+ *            with E = 1: all rows
+ *   Y        MOE_DTYPE_BF16 / F16 / F32 [rows, N], row stride ldy (elements).  Rows of no
+ *            group are left as they were, or set to zero where zero_tail != 0
+ * Products and sums in fp32, one rounding to the output type.  E <= 1024.
+ */
+int moe_fp8_gemm(const void* A, int64_t lda, const float* a_scale, int64_t as_row, int64_t as_k, const void* B,
+                 const float* b_scale, const int32_t* offsets, int64_t rows, int K, int N, int E, void* Y, int64_t ldy,
+                 int out_dtype, int zero_tail, int32_t* status, void* stream);
+
 /* ---- expert grouped GEMM (tcgen05 / TMEM / TMA) -----------------------------------
  * Replaces kernels/grouped_gemm_baseline.py:14-57, kernels/grouped_gemm_tilelang.py:119-214
  * and the expert matmuls of kernels/fusedmoe_baseline.py:93-103,148-158 /

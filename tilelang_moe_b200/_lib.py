@@ -29,6 +29,10 @@ SIGNATURES = {
     "moe_permute": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _i32, _vp, _vp]),
     "moe_unpermute": (_i32, [_vp, _i64, _vp, _vp, _vp, _i64, _i32, _i64, _i32, _vp, _vp]),
     "moe_unpermute_grad": (_i32, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i32, _i64, _i32, _vp, _vp, _vp]),
+    "moe_fp8_quantize_rows": (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp]),
+    "moe_fp8_silu_mul": (_i32, [_vp, _i64, _vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp]),
+    "moe_fp8_quantize_blocks": (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp]),
+    "moe_fp8_gemm": (_i32, [_vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp, _i64, _i32, _i32, _vp, _vp]),
     "moe_grouped_gemm": (_i32, [_i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _vp, _vp]),
     "moe_grouped_gemm_gathered": (_i32, [_i32, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64,
                                          _i32, _i32, _i32, _i32, _vp, _vp]),

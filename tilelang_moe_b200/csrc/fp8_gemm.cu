@@ -1,0 +1,392 @@
+// 8-bit GEMM with a scale for each block of 128, dense or grouped by expert, for sm_100a.
+//
+//   Y[m, n] = sum over kb of  sa[m, kb] * sb[n / 128, kb] * ( sum over the 128 k of block kb of  A[m, k] * B[n, k] )
+//
+// A [rows, K] and B [E, N, K] are e4m3, the inner sums are taken by tcgen05.mma (kind::f8f6f4, fp32 accumulators in tensor
+// memory), and because the scales change every 128 k, each block's sum leaves tensor memory and is added, scaled, to fp32
+// accumulators in registers:
+//
+//   warp 0      TMA producer: per k-block one A box (128 rows x 128 bytes) and one B box (BN rows), 128-byte swizzle, into a
+//               ring of shared-memory stages;
+//   warp 1      MMA issuer: four instructions (K = 32) per k-block into one of two accumulators in tensor memory, in turn;
+//   warps 2..9  one tile row and half of the tile's columns per thread: acc += (sa * sb) * block sum, while the other
+//               accumulator is being filled; after the last block convert and store.
+//
+// K need not be a multiple of 128: TMA fills what lies behind it with zeros.  Rows of a tile behind its group are computed
+// and not stored.  Every barrier wait is bounded in time, as in the 16-bit kernels.
+#include "sm100.cuh"
+
+#include <cuda_fp16.h>
+
+namespace moe {
+namespace gemm8 {
+
+using namespace moe::gemm;
+
+constexpr int BM = 128;
+constexpr int BK = 128;                // bytes = elements: one swizzle row, one scale block
+constexpr int UMMA_K = 32;
+constexpr int NUM_THREADS = 320;
+constexpr int EPI_WARPS = 8;
+constexpr int MAX_E = 1024;
+
+template <int BN>
+struct Cfg {
+  static constexpr int A_BYTES = BM * BK;
+  static constexpr int B_BYTES = BN * BK;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int STAGES = (192 * 1024) / STAGE_BYTES;     // BN = 256: 4, 128: 6, 64: 8
+  static constexpr int TMEM_COLS = 2 * BN;
+  static constexpr int BAR_OFFSET = STAGES * STAGE_BYTES;
+  static constexpr int SLOT_OFFSET = BAR_OFFSET + (2 * STAGES + 5) * 8;
+  static constexpr int TABLE_OFFSET = (SLOT_OFFSET + 16 + 15) & ~15;
+  static constexpr int SMEM_BYTES = TABLE_OFFSET + 2 * (MAX_E + 1) * 4 + 1024;    // + alignment slack
+  static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+};
+
+struct Params {
+  const float* sa;
+  int64_t sa_row, sa_k;          // strides
+  const float* sb;               // [E, ceil(N / 128), ceil(K / 128)]
+  const int32_t* offsets;        // null: one group of all rows
+  void* Y;
+  int64_t ldy;
+  int rows, K, N, E;
+  int n_tiles, k_blocks, n_blocks;
+  int out;                       // MOE_DTYPE_*
+  int vec_store;                 // rows of Y take 16-byte stores
+  int zero_tail;                 // rows of no group are set to zero
+  int32_t* status;
+};
+
+__device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D fp32 (bit 4), A and B e4m3 (formats 0), both K-major
+__host__ __device__ constexpr uint32_t make_idesc(int m, int n) {
+  return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// 32 lanes x 16 consecutive fp32 columns, and the wait for them; the registers pass through the wait, so that no use of
+// them moves above it
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld_wait16(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :: "memory");
+}
+
+struct Tile {
+  int e, row0, row_end, n_tile;
+};
+// tstart[e] = row tiles of the groups before e.  Tile ids: group, then column tile, then row tile, so that CTAs side by side
+// read one B tile.
+__device__ __forceinline__ Tile decode_tile(int id, const int32_t* tstart, const int32_t* offs, int E, int NT) {
+  int lo = 0, hi = E - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (tstart[mid + 1] * NT > id) hi = mid; else lo = mid + 1;
+  }
+  const int local = id - tstart[lo] * NT, mt = tstart[lo + 1] - tstart[lo];
+  Tile t;
+  t.e = lo;
+  t.n_tile = local / mt;
+  t.row0 = offs[lo] + (local - t.n_tile * mt) * BM;
+  t.row_end = offs[lo + 1];
+  return t;
+}
+__device__ __forceinline__ int group_tiles(const int32_t* offs, int e) { return max(0, offs[e + 1] - offs[e] + BM - 1) / BM; }
+__device__ __forceinline__ void tile_prefix(int32_t* tstart, const int32_t* offs, int E, int lane) {
+  const int per = (E + 31) / 32;
+  const int e_lo = min(E, lane * per), e_hi = min(E, e_lo + per);
+  int sum = 0;
+  for (int e = e_lo; e < e_hi; ++e) sum += group_tiles(offs, e);
+  int inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  int run = inc - sum;
+  for (int e = e_lo; e < e_hi; ++e) { tstart[e] = run; run += group_tiles(offs, e); }
+  if (lane == 31) tstart[E] = inc;
+}
+
+__device__ __forceinline__ uint32_t pack16(float a, float b, int out) {
+  if (out == MOE_DTYPE_F16) { __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<uint32_t*>(&h); }
+  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ uint16_t one16(float a, int out) {
+  return out == MOE_DTYPE_F16 ? __half_as_ushort(__float2half_rn(a)) : __bfloat16_as_ushort(__float2bfloat16_rn(a));
+}
+
+template <int BN>
+__global__ void __launch_bounds__(NUM_THREADS, 1)
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
+  using C = Cfg<BN>;
+  constexpr int STAGES = C::STAGES, COLS = BN / 2;       // COLS: columns of an epilogue thread
+  extern __shared__ unsigned char smem_dyn[];
+  // the swizzle pattern needs 1024-byte aligned stage buffers
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_dyn) + 1023) & ~(uintptr_t)1023);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::BAR_OFFSET);
+  // bars[0..S) full, [S..2S) empty, [2S..2S+2) tmem_full, [2S+2..2S+4) tmem_empty, [2S+4] drain
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::SLOT_OFFSET);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::SLOT_OFFSET + 8);
+  int32_t* tstart = reinterpret_cast<int32_t*>(smem + C::TABLE_OFFSET);
+  int32_t* offs = tstart + (MAX_E + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
+  const uint32_t tfull0 = smem_u32(bars + 2 * STAGES), tempty0 = smem_u32(bars + 2 * STAGES + 2);
+  const uint32_t drain_bar = smem_u32(bars + 2 * STAGES + 4);
+  const int E = p.E, NT = p.n_tiles, NKB = p.k_blocks;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
+    for (int b = 0; b < 2; ++b) { mbar_init(tfull0 + 8 * b, 1); mbar_init(tempty0 + 8 * b, EPI_WARPS); }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_tmap(&tmA);
+    prefetch_tmap(&tmB);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  // a table that is no prefix sum leaves every access inside the tensors: starts and ends are cut to [0, rows]
+  for (int e = threadIdx.x; e <= E; e += blockDim.x) offs[e] = p.offsets ? min(max(p.offsets[e], 0), p.rows) : (e == 0 ? 0 : p.rows);
+  __syncthreads();
+  if (warp == 2) tile_prefix(tstart, offs, E, lane);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int total_tiles = tstart[E] * NT;
+
+  if (warp == 0) {
+    // ===================================================================== TMA producer
+    int stage = 0;
+    uint32_t phase = 0, issued = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
+      const Tile t = decode_tile(tile, tstart, offs, E, NT);
+      for (int kb = 0; kb < NKB; ++kb) {
+        if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, abort_flag, p.status, 31)) { ok = false; break; }
+        if (lane == 0) {
+          const uint32_t full = full0 + 8 * stage;
+          const uint32_t sa = smem_u32(smem + stage * C::STAGE_BYTES);
+          mbar_arrive_expect_tx(full, C::STAGE_BYTES);
+          tma_load_2d(sa, &tmA, full, kb * BK, t.row0);
+          tma_load_3d(sa + C::A_BYTES, &tmB, full, kb * BK, t.n_tile * BN, t.e);
+        }
+        __syncwarp();
+        ++issued;
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+    if (!ok) {
+      // let the copies already issued land before the CTA retires its shared memory
+      const uint32_t first = issued > (uint32_t)STAGES ? issued - STAGES : 0;
+      for (uint32_t j = first; j < issued; ++j) mbar_wait_drain(full0 + 8 * (j % STAGES), (j / STAGES) & 1, DRAIN_LIMIT_NS);
+    }
+  } else if (warp == 1) {
+    // ===================================================================== MMA issuer
+    constexpr uint32_t idesc = make_idesc(BM, BN);
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
+      for (int kb = 0; kb < NKB; ++kb) {
+        if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, p.status, 32)) { ok = false; break; }
+        if (!mbar_wait(full0 + 8 * stage, phase, abort_flag, p.status, 33)) { ok = false; break; }
+        tc_fence_after();
+        if (lane == 0) {
+          const uint32_t sa = smem_u32(smem + stage * C::STAGE_BYTES);
+          const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + C::A_BYTES);
+#pragma unroll
+          for (int k = 0; k < BK / UMMA_K; ++k)       // 32 bytes further inside the swizzle row: +2 in the (addr >> 4) field
+            umma_e4m3(tmem_base + (uint32_t)(acc * BN), adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, k != 0 ? 1u : 0u);
+          umma_commit(empty0 + 8 * stage);
+          umma_commit(tfull0 + 8 * acc);
+        }
+        __syncwarp();
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      }
+    }
+    if (!ok) {
+      // wait (bounded) until the tensor-core work issued so far has retired, so that tensor memory can be freed
+      if (lane == 0) umma_commit(drain_bar);
+      __syncwarp();
+      mbar_wait_drain(drain_bar, 0, DRAIN_LIMIT_NS);
+    }
+  } else {
+    // ===================================================================== scaled accumulation and store (warps 2..9)
+    const int q = warp & 3;                           // tensor-memory lane quarter this warp may read
+    const int half = (warp - 2) >> 2;                 // its half of the columns
+    const int out = p.out;
+    const size_t el = out == MOE_DTYPE_F32 ? 4 : 2;
+    int buf = 0;
+    uint32_t buf_phase = 0;
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
+      const Tile t = decode_tile(tile, tstart, offs, E, NT);
+      const int row = t.row0 + q * 32 + lane, col0 = t.n_tile * BN + half * COLS;
+      const bool row_ok = row < t.row_end;
+      const float* sa = p.sa + (row_ok ? (int64_t)row * p.sa_row : 0);
+      // columns behind N have no scale block of their own: the last one stands in, nothing of them is stored
+      const float* sb = p.sb + ((int64_t)t.e * p.n_blocks + min(col0 / 128, p.n_blocks - 1)) * NKB;
+      float acc[COLS];
+#pragma unroll
+      for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
+      float s_next = sa[0] * sb[0];
+      for (int kb = 0; kb < NKB; ++kb) {
+        const float s = s_next;
+        if (kb + 1 < NKB) s_next = sa[(kb + 1) * p.sa_k] * sb[kb + 1];
+        if (!mbar_wait(tfull0 + 8 * buf, buf_phase, abort_flag, p.status, 34)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + half * COLS);
+#pragma unroll
+        for (int c = 0; c < COLS / 16; ++c) {
+          uint32_t v[16];
+          tmem_ld16(taddr + c * 16, v);
+          tmem_ld_wait16(v);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(__uint_as_float(v[j]), s, acc[c * 16 + j]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tempty0 + 8 * buf);
+        if (++buf == 2) { buf = 0; buf_phase ^= 1; }
+      }
+      if (!ok || !row_ok) continue;
+      unsigned char* y = reinterpret_cast<unsigned char*>(p.Y) + ((int64_t)row * p.ldy + col0) * el;
+      if (p.vec_store) {
+        if (out == MOE_DTYPE_F32) {
+#pragma unroll
+          for (int j = 0; j < COLS; j += 4)
+            if (col0 + j < p.N) *reinterpret_cast<float4*>(y + j * 4) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < COLS; j += 8)
+            if (col0 + j < p.N)
+              *reinterpret_cast<uint4*>(y + j * 2) = make_uint4(pack16(acc[j], acc[j + 1], out), pack16(acc[j + 2], acc[j + 3], out),
+                                                                pack16(acc[j + 4], acc[j + 5], out), pack16(acc[j + 6], acc[j + 7], out));
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < COLS; ++j) {
+          if (col0 + j < p.N) {
+            if (out == MOE_DTYPE_F32) reinterpret_cast<float*>(y)[j] = acc[j];
+            else reinterpret_cast<uint16_t*>(y)[j] = one16(acc[j], out);
+          }
+        }
+      }
+    }
+    if (p.zero_tail) {
+      const int64_t ahead = offs[0], behind = offs[E];     // rows of no group: those before the first one too
+      for (int64_t i = (int64_t)blockIdx.x * EPI_WARPS + (warp - 2); i < ahead + p.rows - behind; i += (int64_t)gridDim.x * EPI_WARPS) {
+        const int64_t r = i < ahead ? i : behind + i - ahead;
+        unsigned char* y = reinterpret_cast<unsigned char*>(p.Y) + r * p.ldy * el;
+        for (int c = lane; c < p.N; c += 32) {
+          if (el == 4) reinterpret_cast<uint32_t*>(y)[c] = 0u;
+          else reinterpret_cast<uint16_t*>(y)[c] = 0;
+        }
+      }
+    }
+  }
+
+  // ---- teardown
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------------------ host side
+// 8-bit tensor [d2][d1][d0] (d0 contiguous, rows ld1 bytes apart), box [1][box1][128], 128-byte swizzle, zeros out of bounds
+static int make_tmap8(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t ld1, uint32_t box1) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return fail(MOE_ERR_DEVICE, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[3] = {d0, d1, d2};
+  cuuint64_t strides[2] = {ld1, ld1 * d1};
+  cuuint32_t box[3] = {(cuuint32_t)BK, box1, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, d2 > 0 ? 3 : 2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(MOE_ERR_ARG, "cuTensorMapEncodeTiled failed with %d (dims %llu,%llu,%llu row %llu box1 %u)", (int)r, (unsigned long long)d0,
+                (unsigned long long)d1, (unsigned long long)d2, (unsigned long long)ld1, box1);
+  return MOE_OK;
+}
+
+template <int BN>
+static int launch(const void* A, int64_t lda, const void* B, Params p, int sms, cudaStream_t st) {
+  using C = Cfg<BN>;
+  static std::atomic<bool> attr_set[64];
+  int rc = allow_dynamic_smem(fp8_gemm_kernel<BN>, C::SMEM_BYTES, attr_set);
+  if (rc) return rc;
+  p.n_tiles = (p.N + BN - 1) / BN;
+  const int64_t bound = ((int64_t)p.rows / BM + p.E) * p.n_tiles;
+  if (bound > 0x7FFFFFFFll) return fail(MOE_ERR_UNSUPPORTED, "fp8_gemm: too many tiles");
+  CUtensorMap tA, tB;
+  rc = make_tmap8(&tA, A, (uint64_t)p.K, (uint64_t)p.rows, 0, (uint64_t)lda, (uint32_t)BM);
+  if (rc) return rc;
+  rc = make_tmap8(&tB, B, (uint64_t)p.K, (uint64_t)p.N, (uint64_t)p.E, (uint64_t)p.K, (uint32_t)BN);
+  if (rc) return rc;
+  MOE_LAUNCH("fp8_gemm_kernel", fp8_gemm_kernel<BN>, (unsigned)(bound < sms ? bound : sms), NUM_THREADS, C::SMEM_BYTES, st, false, tA, tB, p);
+  return MOE_OK;
+}
+
+}  // namespace gemm8
+}  // namespace moe
+
+// ====================================================================================
+extern "C" int moe_fp8_gemm(const void* A, int64_t lda, const float* a_scale, int64_t as_row, int64_t as_k, const void* B,
+                            const float* b_scale, const int32_t* offsets, int64_t rows, int K, int N, int E, void* Y, int64_t ldy,
+                            int out_dtype, int zero_tail, int32_t* status, void* stream) {
+  using namespace moe;
+  using namespace moe::gemm8;
+  if (out_dtype < 0 || out_dtype > MOE_DTYPE_F32) return fail(MOE_ERR_ARG, "fp8_gemm: unknown output type %d", out_dtype);
+  if (rows < 0 || K < 16 || K % 16 || N < 1 || E < 1)
+    return fail(MOE_ERR_ARG, "fp8_gemm: bad shape rows=%lld K=%d N=%d E=%d (K a multiple of 16)", (long long)rows, K, N, E);
+  if (E > MAX_E) return fail(MOE_ERR_UNSUPPORTED, "fp8_gemm: E=%d exceeds %d", E, MAX_E);
+  if (!offsets && E != 1) return fail(MOE_ERR_ARG, "fp8_gemm: several groups need an offsets table");
+  if (rows == 0) return MOE_OK;
+  if (rows > 0x7FFFFF00ll) return fail(MOE_ERR_UNSUPPORTED, "fp8_gemm: too many rows");
+  if (!A || !a_scale || !B || !b_scale || !Y) return fail(MOE_ERR_ARG, "fp8_gemm: null pointer");
+  if ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(B)) & 15) return fail(MOE_ERR_ARG, "fp8_gemm: A and B must be 16-byte aligned");
+  if (lda < K || lda % 16) return fail(MOE_ERR_ARG, "fp8_gemm: lda=%lld must be at least K and a multiple of 16", (long long)lda);
+  if (as_row < 0 || as_k < 0) return fail(MOE_ERR_ARG, "fp8_gemm: negative stride of the row scales");
+  if (ldy < N) return fail(MOE_ERR_ARG, "fp8_gemm: ldy=%lld is less than N", (long long)ldy);
+  DeviceInfo dev;
+  int rc = current_device_info(&dev);
+  if (rc) return rc;
+  Params p;
+  p.sa = a_scale; p.sa_row = as_row; p.sa_k = as_k; p.sb = b_scale; p.offsets = offsets;
+  p.Y = Y; p.ldy = ldy; p.rows = (int)rows; p.K = K; p.N = N; p.E = E;
+  p.n_tiles = 0; p.k_blocks = (K + BK - 1) / BK; p.n_blocks = (N + 127) / 128;
+  p.out = out_dtype; p.zero_tail = zero_tail != 0 && offsets != nullptr; p.status = status;
+  const int64_t el = out_dtype == MOE_DTYPE_F32 ? 4 : 2;
+  p.vec_store = !(reinterpret_cast<uintptr_t>(Y) & 15) && (ldy * el) % 16 == 0 && (N * el) % 16 == 0;
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  return launch<256>(A, lda, B, p, dev.sm_count, st);
+}

@@ -27,6 +27,7 @@ import torch
 
 from .. import layer as _layer
 from .. import ops as _ops
+from ..fp8 import fp8_gemm, fp8_grouped_gemm, fp8_quantize, fp8_quantize_blocks, fp8_silu_mul
 from ..permute import MoESort, moe_permute, moe_sort, moe_unpermute
 
 __all__ = [
@@ -34,6 +35,8 @@ __all__ = [
     "FusedMoETileLang", "FusedMoE", "generate_fusedmoe_inputs", "route_histogram", "mhc_pre", "mhc_post",
     # operators the reference does not have: tokens sorted by expert and back, with gradients
     "MoESort", "moe_sort", "moe_permute", "moe_unpermute",
+    # ... and 8-bit operands with the products of them
+    "fp8_quantize", "fp8_quantize_blocks", "fp8_silu_mul", "fp8_gemm", "fp8_grouped_gemm",
     # the reference's other public names (its strategy variants and its PyTorch baselines): the same operator each
     "topk_softmax_fused", "topk_softmax_selection", "topk_softmax_sonic", "topk_softmax_bitonic",
     "topk_softmax_separate", "topk_softmax_separate_compiled", "topk_softmax_tilelang_separate", "topk_radix_tilelang",
