@@ -71,23 +71,41 @@ __device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint
 __host__ __device__ constexpr uint32_t make_idesc(int m, int n) {
   return (1u << 4) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// 32 lanes x 16 consecutive fp32 columns, and the wait for them; the registers pass through the wait, so that no use of
-// them moves above it
-__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+// Two fp32 in one 64-bit register pair.  The scaled additions are fma.rn.f32x2: plain fma instructions take the tensor cores'
+// time.  Measured, clocks for the four instructions of a k-block (128 x 256) beside accumulating warps that never wait: alone
+// 518, beside fma only 1520, beside fma.rn.f32x2 only 571; with the tensor-memory loads 916 and 670.
+typedef unsigned long long f32x2;
+// 32 lanes x 16 consecutive fp32 columns of tensor memory, waited for, in pairs: one statement, so that no use of the values
+// can be moved above the wait
+__device__ __forceinline__ void tmem_ld16_pairs(uint32_t taddr, f32x2 (&r)[8]) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      "{\n\t.reg .b32 t<16>;\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {t0, t1, t2, t3, t4, t5, t6, t7, t8, t9, t10, t11, t12, t13, t14, t15}, [%8];\n\t"
+      "tcgen05.wait::ld.sync.aligned;\n\t"
+      "mov.b64 %0, {t0, t1};\n\t"
+      "mov.b64 %1, {t2, t3};\n\t"
+      "mov.b64 %2, {t4, t5};\n\t"
+      "mov.b64 %3, {t6, t7};\n\t"
+      "mov.b64 %4, {t8, t9};\n\t"
+      "mov.b64 %5, {t10, t11};\n\t"
+      "mov.b64 %6, {t12, t13};\n\t"
+      "mov.b64 %7, {t14, t15};\n\t"
+      "}"
+      : "=l"(r[0]), "=l"(r[1]), "=l"(r[2]), "=l"(r[3]), "=l"(r[4]), "=l"(r[5]), "=l"(r[6]), "=l"(r[7])
       : "r"(taddr)
       : "memory");
 }
-__device__ __forceinline__ void tmem_ld_wait16(uint32_t (&r)[16]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                 "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-               :: "memory");
+__device__ __forceinline__ f32x2 pair_of(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
+__device__ __forceinline__ float2 unpair(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ void fma2(f32x2& acc, f32x2 v, f32x2 s) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s)); }
 
 struct Tile {
   int e, row0, row_end, n_tile;
@@ -108,7 +126,9 @@ __device__ __forceinline__ Tile decode_tile(int id, const int32_t* tstart, const
   t.row_end = offs[lo + 1];
   return t;
 }
-__device__ __forceinline__ int group_tiles(const int32_t* offs, int e) { return max(0, offs[e + 1] - offs[e] + BM - 1) / BM; }
+__device__ __forceinline__ int group_tiles(const int32_t* offs, int e) {
+  return max(0, offs[e + 1] - offs[e] + BM - 1) / BM;
+}
 __device__ __forceinline__ void tile_prefix(int32_t* tstart, const int32_t* offs, int E, int lane) {
   const int per = (E + 31) / 32;
   const int e_lo = min(E, lane * per), e_hi = min(E, e_lo + per);
@@ -125,13 +145,54 @@ __device__ __forceinline__ void tile_prefix(int32_t* tstart, const int32_t* offs
   if (lane == 31) tstart[E] = inc;
 }
 
-__device__ __forceinline__ uint32_t pack16(float a, float b, int out) {
-  if (out == MOE_DTYPE_F16) { __half2 h = __floats2half2_rn(a, b); return *reinterpret_cast<uint32_t*>(&h); }
-  __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+__device__ __forceinline__ uint32_t pack16(f32x2 pair, int out) {
+  const float2 v = unpair(pair);
+  if (out == MOE_DTYPE_F16) { __half2 h = __floats2half2_rn(v.x, v.y); return *reinterpret_cast<uint32_t*>(&h); }
+  __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
   return *reinterpret_cast<uint32_t*>(&h);
 }
 __device__ __forceinline__ uint16_t one16(float a, int out) {
   return out == MOE_DTYPE_F16 ? __half_as_ushort(__float2half_rn(a)) : __bfloat16_as_ushort(__float2bfloat16_rn(a));
+}
+
+// columns [col0, col0 + COLS) of one row, those below N, rounded to the output type
+template <int COLS>
+__device__ __forceinline__ void store_row(const Params& p, int64_t row, int col0, const f32x2 (&acc)[COLS / 2]) {
+  const int out = p.out;
+  unsigned char* y = reinterpret_cast<unsigned char*>(p.Y) + (row * p.ldy + col0) * (out == MOE_DTYPE_F32 ? 4 : 2);
+  if (p.vec_store) {
+    if (out == MOE_DTYPE_F32) {
+#pragma unroll
+      for (int j = 0; j < COLS / 2; j += 2)
+        if (col0 + 2 * j < p.N) *reinterpret_cast<ulonglong2*>(y + j * 8) = make_ulonglong2(acc[j], acc[j + 1]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < COLS / 2; j += 4)
+        if (col0 + 2 * j < p.N)
+          *reinterpret_cast<uint4*>(y + j * 4) = make_uint4(pack16(acc[j], out), pack16(acc[j + 1], out), pack16(acc[j + 2], out), pack16(acc[j + 3], out));
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < COLS; ++j) {
+      const float a = j & 1 ? unpair(acc[j / 2]).y : unpair(acc[j / 2]).x;
+      if (col0 + j < p.N) {
+        if (out == MOE_DTYPE_F32) reinterpret_cast<float*>(y)[j] = a;
+        else reinterpret_cast<uint16_t*>(y)[j] = one16(a, out);
+      }
+    }
+  }
+}
+
+// rows of no group, before the first one and behind the last, set to zero; warps w of n
+__device__ __forceinline__ void zero_rows(const Params& p, int64_t ahead, int64_t behind, int64_t w, int64_t n, int lane) {
+  for (int64_t i = w; i < ahead + p.rows - behind; i += n) {
+    const int64_t r = i < ahead ? i : behind + i - ahead;
+    unsigned char* y = reinterpret_cast<unsigned char*>(p.Y) + r * p.ldy * (p.out == MOE_DTYPE_F32 ? 4 : 2);
+    for (int c = lane; c < p.N; c += 32) {
+      if (p.out == MOE_DTYPE_F32) reinterpret_cast<uint32_t*>(y)[c] = 0u;
+      else reinterpret_cast<uint16_t*>(y)[c] = 0;
+    }
+  }
 }
 
 template <int BN>
@@ -205,42 +266,42 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       for (uint32_t j = first; j < issued; ++j) mbar_wait_drain(full0 + 8 * (j % STAGES), (j / STAGES) & 1, DRAIN_LIMIT_NS);
     }
   } else if (warp == 1) {
-    // ===================================================================== MMA issuer
-    constexpr uint32_t idesc = make_idesc(BM, BN);
-    int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
-    bool ok = true;
-    for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
-      for (int kb = 0; kb < NKB; ++kb) {
-        if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, p.status, 32)) { ok = false; break; }
-        if (!mbar_wait(full0 + 8 * stage, phase, abort_flag, p.status, 33)) { ok = false; break; }
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t sa = smem_u32(smem + stage * C::STAGE_BYTES);
-          const uint64_t adesc = make_smem_desc(sa), bdesc = make_smem_desc(sa + C::A_BYTES);
+    // ===================================================================== MMA issuer: one thread
+    // Nothing but the waits and the instructions between two k-blocks: the tensor cores queue few instructions, and what
+    // the issuer takes between two blocks beyond that they stand still.
+    if (lane == 0) {
+      constexpr uint32_t idesc = make_idesc(BM, BN);
+      const uint64_t adesc0 = make_smem_desc(smem_u32(smem)), bdesc0 = make_smem_desc(smem_u32(smem) + C::A_BYTES);
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
+        for (int kb = 0; kb < NKB; ++kb) {
+          if (!mbar_wait(full0 + 8 * stage, phase, abort_flag, p.status, 33)) { ok = false; break; }
+          if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, p.status, 32)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t adesc = adesc0 + (uint64_t)(stage * (C::STAGE_BYTES >> 4)), bdesc = bdesc0 + (uint64_t)(stage * (C::STAGE_BYTES >> 4));
+          const uint32_t d = tmem_base + (uint32_t)(acc * BN);
 #pragma unroll
           for (int k = 0; k < BK / UMMA_K; ++k)       // 32 bytes further inside the swizzle row: +2 in the (addr >> 4) field
-            umma_e4m3(tmem_base + (uint32_t)(acc * BN), adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, k != 0 ? 1u : 0u);
-          umma_commit(empty0 + 8 * stage);
+            umma_e4m3(d, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, k != 0 ? 1u : 0u);
           umma_commit(tfull0 + 8 * acc);
+          umma_commit(empty0 + 8 * stage);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          if (++acc == 2) { acc = 0; acc_phase ^= 1; }
         }
-        __syncwarp();
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
-        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+      }
+      if (!ok) {
+        // wait (bounded) until the tensor-core work issued so far has retired, so that tensor memory can be freed
+        umma_commit(drain_bar);
+        mbar_wait_drain(drain_bar, 0, DRAIN_LIMIT_NS);
       }
     }
-    if (!ok) {
-      // wait (bounded) until the tensor-core work issued so far has retired, so that tensor memory can be freed
-      if (lane == 0) umma_commit(drain_bar);
-      __syncwarp();
-      mbar_wait_drain(drain_bar, 0, DRAIN_LIMIT_NS);
-    }
+    __syncwarp();
   } else {
     // ===================================================================== scaled accumulation and store (warps 2..9)
     const int q = warp & 3;                           // tensor-memory lane quarter this warp may read
     const int half = (warp - 2) >> 2;                 // its half of the columns
-    const int out = p.out;
-    const size_t el = out == MOE_DTYPE_F32 ? 4 : 2;
     int buf = 0;
     uint32_t buf_phase = 0;
     bool ok = true;
@@ -251,9 +312,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       const float* sa = p.sa + (row_ok ? (int64_t)row * p.sa_row : 0);
       // columns behind N have no scale block of their own: the last one stands in, nothing of them is stored
       const float* sb = p.sb + ((int64_t)t.e * p.n_blocks + min(col0 / 128, p.n_blocks - 1)) * NKB;
-      float acc[COLS];
+      f32x2 acc[COLS / 2];
 #pragma unroll
-      for (int j = 0; j < COLS; ++j) acc[j] = 0.f;
+      for (int j = 0; j < COLS / 2; ++j) acc[j] = 0ull;
       float s_next = sa[0] * sb[0];
       for (int kb = 0; kb < NKB; ++kb) {
         const float s = s_next;
@@ -261,54 +322,22 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         if (!mbar_wait(tfull0 + 8 * buf, buf_phase, abort_flag, p.status, 34)) { ok = false; break; }
         tc_fence_after();
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + half * COLS);
+        const f32x2 s2 = pair_of(s, s);
 #pragma unroll
         for (int c = 0; c < COLS / 16; ++c) {
-          uint32_t v[16];
-          tmem_ld16(taddr + c * 16, v);
-          tmem_ld_wait16(v);
+          f32x2 v[8];
+          tmem_ld16_pairs(taddr + c * 16, v);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(__uint_as_float(v[j]), s, acc[c * 16 + j]);
+          for (int j = 0; j < 8; ++j) fma2(acc[c * 8 + j], v[j], s2);
         }
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(tempty0 + 8 * buf);
         if (++buf == 2) { buf = 0; buf_phase ^= 1; }
       }
-      if (!ok || !row_ok) continue;
-      unsigned char* y = reinterpret_cast<unsigned char*>(p.Y) + ((int64_t)row * p.ldy + col0) * el;
-      if (p.vec_store) {
-        if (out == MOE_DTYPE_F32) {
-#pragma unroll
-          for (int j = 0; j < COLS; j += 4)
-            if (col0 + j < p.N) *reinterpret_cast<float4*>(y + j * 4) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < COLS; j += 8)
-            if (col0 + j < p.N)
-              *reinterpret_cast<uint4*>(y + j * 2) = make_uint4(pack16(acc[j], acc[j + 1], out), pack16(acc[j + 2], acc[j + 3], out),
-                                                                pack16(acc[j + 4], acc[j + 5], out), pack16(acc[j + 6], acc[j + 7], out));
-        }
-      } else {
-#pragma unroll
-        for (int j = 0; j < COLS; ++j) {
-          if (col0 + j < p.N) {
-            if (out == MOE_DTYPE_F32) reinterpret_cast<float*>(y)[j] = acc[j];
-            else reinterpret_cast<uint16_t*>(y)[j] = one16(acc[j], out);
-          }
-        }
-      }
+      if (ok && row_ok) store_row<COLS>(p, row, col0, acc);
     }
-    if (p.zero_tail) {
-      const int64_t ahead = offs[0], behind = offs[E];     // rows of no group: those before the first one too
-      for (int64_t i = (int64_t)blockIdx.x * EPI_WARPS + (warp - 2); i < ahead + p.rows - behind; i += (int64_t)gridDim.x * EPI_WARPS) {
-        const int64_t r = i < ahead ? i : behind + i - ahead;
-        unsigned char* y = reinterpret_cast<unsigned char*>(p.Y) + r * p.ldy * el;
-        for (int c = lane; c < p.N; c += 32) {
-          if (el == 4) reinterpret_cast<uint32_t*>(y)[c] = 0u;
-          else reinterpret_cast<uint16_t*>(y)[c] = 0;
-        }
-      }
-    }
+    if (p.zero_tail) zero_rows(p, offs[0], offs[E], (int64_t)blockIdx.x * EPI_WARPS + (warp - 2), (int64_t)gridDim.x * EPI_WARPS, lane);
   }
 
   // ---- teardown
