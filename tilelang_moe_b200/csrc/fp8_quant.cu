@@ -10,10 +10,7 @@
 //
 // Bound by memory: an element is read once (2 or 4 bytes, twice that for SiLU) and written once (1 byte), and the group's
 // maximum is taken on the registers that its values stay in.
-#include "common.cuh"
-
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
+#include "vec.cuh"
 
 namespace moe {
 namespace fp8 {
@@ -22,21 +19,6 @@ constexpr int G = 128;               // elements that share a scale along a row
 constexpr float TOP = 448.0f;
 constexpr uint32_t TINY_BITS = 0x0D800000u;   // 2^-100: 448 / top and top / 448 stay normal numbers
 
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-
-template <class T, int V>
-struct alignas(V) Pack {
-  static constexpr int N = V / (int)sizeof(T);
-  T e[N];
-};
-template <int N> struct Bytes;
-template <> struct Bytes<1> { using type = uint8_t; };
-template <> struct Bytes<2> { using type = uint16_t; };
-template <> struct Bytes<4> { using type = uint32_t; };
-template <> struct Bytes<8> { using type = uint2; };
-
 // two fp32 -> two e4m3 in 16 bits, the first in the lower byte
 __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
   uint16_t r;
@@ -44,7 +26,7 @@ __device__ __forceinline__ uint32_t e4m3x2(float a, float b) {
   return r;
 }
 template <int N>
-__device__ __forceinline__ typename Bytes<N>::type quantize(const float* x, float inv) {
+__device__ __forceinline__ Raw<N> quantize(const float* x, float inv) {
   if constexpr (N == 1) return (uint8_t)e4m3x2(x[0] * inv, 0.f);
   else if constexpr (N == 2) return (uint16_t)e4m3x2(x[0] * inv, x[1] * inv);
   else if constexpr (N == 4) return e4m3x2(x[0] * inv, x[1] * inv) | (e4m3x2(x[2] * inv, x[3] * inv) << 16);
@@ -62,65 +44,82 @@ struct RowParams {
   const void* x;         // or the gate
   const void* up;
   int64_t x_stride, up_stride;   // elements
-  int64_t groups;        // rows x groups of a row
-  int K, per_row;        // elements and groups of a row
+  uint32_t groups;       // rows x groups of a row
+  int K;                 // elements of a row
+  FastDiv per_row;       // groups of a row
   uint8_t* q;
   float* scale;
 };
 
-// L lanes hold a group, I vectors of N elements each; a warp takes 32 / L groups at a time, U of them in flight per lane.
+// Groups that a lane has in flight: 64 bytes of loads where a group is one vector per lane, all of the group otherwise.
+template <class T, int V, bool SWIGLU>
+struct RowShape {
+  static constexpr int N = V / (int)sizeof(T);                  // elements of a vector
+  static constexpr int L = G / N < 32 ? G / N : 32;             // lanes of a group
+  static constexpr int I = G / (N * L);                         // vectors of a lane and group
+  static constexpr int U = I > 1 ? 1 : (SWIGLU ? 2 : 4);
+  static constexpr int PER_WARP = U * (32 / L);                 // groups of a warp
+};
+
+// L lanes hold a group, I vectors of N elements each; a warp takes 32 / L groups side by side, U of them in flight per lane.
 // Groups are numbered through all rows, so that short rows fill a warp too.
 template <class T, int V, bool SWIGLU>
 __global__ void __launch_bounds__(256)
 quantize_rows_kernel(const RowParams p) {
-  using P = Pack<T, V>;
-  constexpr int N = P::N, L = G / N < 32 ? G / N : 32, I = G / (N * L), PER_WARP = 32 / L;
-  constexpr int U = I > 1 ? 1 : (SWIGLU ? 2 : 4);
+  using S = RowShape<T, V, SWIGLU>;
+  using P = Raw<V>;
+  constexpr int N = S::N, L = S::L, I = S::I, U = S::U;
   const int lane = threadIdx.x & 31, in = lane % L;
-  const int64_t warps = (int64_t)gridDim.x * 8;
-  for (int64_t first = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) * (U * PER_WARP); first < p.groups; first += warps * (U * PER_WARP)) {
-    P a[U][I], b[U][I];
-    int64_t row[U];
-    int col[U];
+  const uint32_t first = (blockIdx.x * 8 + (threadIdx.x >> 5)) * S::PER_WARP + lane / L;
+  P a[U][I], b[U][I];
+  uint32_t row[U];
+  int col[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t g = first + u * PER_WARP + lane / L;
-      row[u] = g / p.per_row;
-      col[u] = g < p.groups ? (int)(g - row[u] * p.per_row) * G + in * N : p.K;
+  for (int u = 0; u < U; ++u) {
+    const uint32_t g = first + u * (32 / L);
+    row[u] = p.per_row.div(g);
+    col[u] = g < p.groups ? (int)(g - row[u] * p.per_row.d) * G + in * N : p.K;
+    const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)row[u] * p.x_stride;
+    const T* y = SWIGLU ? reinterpret_cast<const T*>(p.up) + (int64_t)row[u] * p.up_stride : x;
 #pragma unroll
-      for (int i = 0; i < I; ++i) {
-        const int c = col[u] + i * L * N;
-        if (c < p.K) {
-          a[u][i] = *reinterpret_cast<const P*>(reinterpret_cast<const T*>(p.x) + row[u] * p.x_stride + c);
-          if (SWIGLU) b[u][i] = *reinterpret_cast<const P*>(reinterpret_cast<const T*>(p.up) + row[u] * p.up_stride + c);
-        }
+    for (int i = 0; i < I; ++i) {
+      const int c = col[u] + i * L * N;
+      if (c < p.K) {
+        a[u][i] = *reinterpret_cast<const P*>(x + c);
+        if (SWIGLU) b[u][i] = *reinterpret_cast<const P*>(y + c);
       }
     }
+  }
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float x[I][N];
-      uint32_t m = 0;
+  for (int u = 0; u < U; ++u) {
+    float x[I][N];
+    uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < I; ++i) {
-        const bool has = col[u] + i * L * N < p.K;
+    for (int i = 0; i < I; ++i) {
+      unpack<T, V>(a[u][i], x[i]);
+      if (SWIGLU) {
+        float y[N];
+        unpack<T, V>(b[u][i], y);
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          x[i][j] = SWIGLU ? silu_mul(to_f32(a[u][i].e[j]), to_f32(b[u][i].e[j])) : to_f32(a[u][i].e[j]);
-          m = max(m, has ? magnitude(x[i][j]) : 0u);
-        }
+        for (int j = 0; j < N; ++j) x[i][j] = silu_mul(x[i][j], y[j]);
       }
+      uint32_t mine = 0;
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-      const float top = __uint_as_float(max(m, TINY_BITS));
-      const float inv = TOP / top;
-#pragma unroll
-      for (int i = 0; i < I; ++i) {
-        const int c = col[u] + i * L * N;
-        if (c < p.K) *reinterpret_cast<typename Bytes<N>::type*>(p.q + row[u] * p.K + c) = quantize<N>(x[i], inv);
-      }
-      const int64_t g = first + u * PER_WARP + lane / L;
-      if (in == 0 && g < p.groups) p.scale[g] = top / TOP;
+      for (int j = 0; j < N; ++j) mine = max(mine, magnitude(x[i][j]));
+      if (col[u] + i * L * N < p.K) m = max(m, mine);
     }
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    const float top = __uint_as_float(max(m, TINY_BITS));
+    const float inv = TOP / top;
+    uint8_t* q = p.q + (int64_t)row[u] * p.K;
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      const int c = col[u] + i * L * N;
+      if (c < p.K) *reinterpret_cast<Raw<N>*>(q + c) = quantize<N>(x[i], inv);
+    }
+    const uint32_t g = first + u * (32 / L);
+    if (in == 0 && g < p.groups) p.scale[g] = top / TOP;
   }
 }
 
@@ -130,8 +129,8 @@ template <class T, int V>
 __global__ void __launch_bounds__(256)
 quantize_blocks_kernel(const T* __restrict__ w, int64_t rows, int K, int row_blocks, int col_blocks, uint8_t* __restrict__ q,
                        float* __restrict__ scale) {
-  using P = Pack<T, V>;
-  constexpr int N = P::N, COLS = G / N, STEP = 256 / COLS, I = G / STEP;    // vectors per row, rows at a time, vectors per thread
+  using P = Raw<V>;
+  constexpr int N = V / (int)sizeof(T), COLS = G / N, STEP = 256 / COLS, I = G / STEP;    // vectors per row, rows at a time, vectors per thread
   __shared__ uint32_t part[8];
   const int c = threadIdx.x % COLS, r0 = threadIdx.x / COLS;
   const int64_t blk = blockIdx.x;
@@ -151,8 +150,10 @@ quantize_blocks_kernel(const T* __restrict__ w, int64_t rows, int K, int row_blo
 #pragma unroll
   for (int i = 0; i < I; ++i)
     if (r0 + i * STEP < left && col < K) {
+      float x[N];
+      unpack<T, V>(v[i], x);
 #pragma unroll
-      for (int j = 0; j < N; ++j) m = max(m, magnitude(to_f32(v[i].e[j])));
+      for (int j = 0; j < N; ++j) m = max(m, magnitude(x[j]));
     }
   m = __reduce_max_sync(0xFFFFFFFFu, m);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
@@ -166,49 +167,44 @@ quantize_blocks_kernel(const T* __restrict__ w, int64_t rows, int K, int row_blo
     const int r = r0 + i * STEP;
     if (r < left && col < K) {
       float x[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j) x[j] = to_f32(v[i].e[j]);
-      *reinterpret_cast<typename Bytes<N>::type*>(q + base + (int64_t)r * K) = quantize<N>(x, inv);
+      unpack<T, V>(v[i], x);
+      *reinterpret_cast<Raw<N>*>(q + base + (int64_t)r * K) = quantize<N>(x, inv);
     }
   }
   if (threadIdx.x == 0) scale[blk] = top / TOP;
 }
 
-static int vec_bytes(uintptr_t all) {
-  int v = 16;
-  while (v > 1 && (all & (uintptr_t)(v - 1))) v >>= 1;
-  return v;
-}
-
 template <class T, int V, bool SWIGLU>
-static void launch_rows(const RowParams& p, int sms, cudaStream_t st) {
-  constexpr int N = V / (int)sizeof(T), L = G / N < 32 ? G / N : 32, U = G / (N * L) > 1 ? 1 : (SWIGLU ? 2 : 4);
-  int64_t grid = ceil_div64(p.groups, 8 * U * (32 / L));
-  if (grid > (int64_t)sms * 8) grid = (int64_t)sms * 8;
-  quantize_rows_kernel<T, V, SWIGLU><<<(unsigned)grid, 256, 0, st>>>(p);
+static void launch_rows(const RowParams& p, cudaStream_t st) {
+  const uint32_t per_cta = 8 * RowShape<T, V, SWIGLU>::PER_WARP;
+  quantize_rows_kernel<T, V, SWIGLU><<<(p.groups + per_cta - 1) / per_cta, 256, 0, st>>>(p);
 }
 
 template <bool SWIGLU>
-static int quantize_rows(const RowParams& p, int64_t rows, int dtype, const char* what, void* stream) {
+static int quantize_rows(const void* x, int64_t x_stride, const void* up, int64_t up_stride, int64_t rows, int K, int dtype, void* q,
+                         float* scale, const char* what, void* stream) {
   if (dtype < 0 || dtype > MOE_DTYPE_F32) return fail(MOE_ERR_ARG, "%s: unknown dtype %d", what, dtype);
-  if (rows < 0 || p.K < 1 || p.x_stride < 0 || p.up_stride < 0) return fail(MOE_ERR_ARG, "%s: bad shape rows=%lld K=%d", what, (long long)rows, p.K);
+  if (rows < 0 || K < 1 || x_stride < 0 || up_stride < 0) return fail(MOE_ERR_ARG, "%s: bad shape rows=%lld K=%d", what, (long long)rows, K);
   if (rows == 0) return MOE_OK;
-  if (!p.x || (SWIGLU && !p.up) || !p.q || !p.scale) return fail(MOE_ERR_ARG, "%s: null pointer", what);
+  const int64_t per_row = ceil_div64(K, G);
+  if (rows > 0x7FFF0000ll / per_row) return fail(MOE_ERR_UNSUPPORTED, "%s: too many groups", what);
+  if (!x || (SWIGLU && !up) || !q || !scale) return fail(MOE_ERR_ARG, "%s: null pointer", what);
   DeviceInfo dev;
   int rc = current_device_info(&dev);
   if (rc) return rc;
   const int w = dtype == MOE_DTYPE_F32 ? 4 : 2;
-  uintptr_t all = reinterpret_cast<uintptr_t>(p.x) | (uintptr_t)(p.x_stride * w) | (uintptr_t)((int64_t)p.K * w);
-  if (SWIGLU) all |= reinterpret_cast<uintptr_t>(p.up) | (uintptr_t)(p.up_stride * w);
+  const RowParams p{x, up, x_stride, up_stride, (uint32_t)(rows * per_row), K, FastDiv((uint32_t)per_row), reinterpret_cast<uint8_t*>(q), scale};
+  uintptr_t all = reinterpret_cast<uintptr_t>(x) | (uintptr_t)(x_stride * w) | (uintptr_t)((int64_t)K * w);
+  if (SWIGLU) all |= reinterpret_cast<uintptr_t>(up) | (uintptr_t)(up_stride * w);
   int V = vec_bytes(all);
   if (V < w) return fail(MOE_ERR_ARG, "%s: rows are not aligned to their element type", what);
   // a vector of V bytes leaves as V / w bytes: the packed 8-bit rows are aligned for it where the base is
-  if (reinterpret_cast<uintptr_t>(p.q) & (uintptr_t)(V / w - 1)) V = w;
+  if (reinterpret_cast<uintptr_t>(q) & (uintptr_t)(V / w - 1)) V = w;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == MOE_DTYPE_F32) V == 16 ? launch_rows<float, 16, SWIGLU>(p, dev.sm_count, st) : launch_rows<float, 4, SWIGLU>(p, dev.sm_count, st);
+  if (dtype == MOE_DTYPE_F32) V == 16 ? launch_rows<float, 16, SWIGLU>(p, st) : launch_rows<float, 4, SWIGLU>(p, st);
 #define MOE_ROWS16(T_)                                                                                             \
-  V == 16 ? launch_rows<T_, 16, SWIGLU>(p, dev.sm_count, st)                                                       \
-          : V >= 4 ? launch_rows<T_, 4, SWIGLU>(p, dev.sm_count, st) : launch_rows<T_, 2, SWIGLU>(p, dev.sm_count, st)
+  V == 16 ? launch_rows<T_, 16, SWIGLU>(p, st)                                                       \
+          : V >= 4 ? launch_rows<T_, 4, SWIGLU>(p, st) : launch_rows<T_, 2, SWIGLU>(p, st)
   else if (dtype == MOE_DTYPE_F16) MOE_ROWS16(__half);
   else MOE_ROWS16(__nv_bfloat16);
 #undef MOE_ROWS16
@@ -223,17 +219,13 @@ static int quantize_rows(const RowParams& p, int64_t rows, int dtype, const char
 extern "C" int moe_fp8_quantize_rows(const void* x, int64_t x_stride, int64_t rows, int K, int dtype, void* q, float* scale,
                                      void* stream) {
   using namespace moe::fp8;
-  const int per_row = K > 0 ? (K + G - 1) / G : 0;
-  const RowParams p{x, nullptr, x_stride, 0, rows * per_row, K, per_row, reinterpret_cast<uint8_t*>(q), scale};
-  return quantize_rows<false>(p, rows, dtype, "fp8_quantize_rows", stream);
+  return quantize_rows<false>(x, x_stride, nullptr, 0, rows, K, dtype, q, scale, "fp8_quantize_rows", stream);
 }
 
 extern "C" int moe_fp8_silu_mul(const void* gate, int64_t gate_stride, const void* up, int64_t up_stride, int64_t rows, int I, int dtype,
                                 void* q, float* scale, void* stream) {
   using namespace moe::fp8;
-  const int per_row = I > 0 ? (I + G - 1) / G : 0;
-  const RowParams p{gate, up, gate_stride, up_stride, rows * per_row, I, per_row, reinterpret_cast<uint8_t*>(q), scale};
-  return quantize_rows<true>(p, rows, dtype, "fp8_silu_mul", stream);
+  return quantize_rows<true>(gate, gate_stride, up, up_stride, rows, I, dtype, q, scale, "fp8_silu_mul", stream);
 }
 
 extern "C" int moe_fp8_quantize_blocks(const void* w, int64_t E, int64_t rows, int K, int dtype, void* q, float* scale, void* stream) {

@@ -10,33 +10,10 @@
 // All of it is bound by memory.  Every kernel goes by tokens, not by sorted rows: a token's row is read once and written to
 // its k places (permute, gradient of unpermute), or its k rows are read and leave as one (unpermute), so nothing is read
 // twice and no sum needs an atomic; the order of every sum is fixed.
-#include "common.cuh"
-
-#include <cuda_fp16.h>
+#include "vec.cuh"
 
 namespace moe {
 namespace perm {
-
-template <int V> struct VecOf;
-template <> struct VecOf<16> { using type = uint4; };
-template <> struct VecOf<8> { using type = uint2; };
-template <> struct VecOf<4> { using type = uint32_t; };
-template <> struct VecOf<2> { using type = uint16_t; };
-template <> struct VecOf<1> { using type = uint8_t; };
-
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void from_f32(float x, float* o) { *o = x; }
-__device__ __forceinline__ void from_f32(float x, __half* o) { *o = __float2half_rn(x); }
-__device__ __forceinline__ void from_f32(float x, __nv_bfloat16* o) { *o = __float2bfloat16_rn(x); }
-
-// V bytes of elements of type T
-template <class T, int V>
-struct alignas(V) Pack {
-  static constexpr int N = V / (int)sizeof(T);
-  T e[N];
-};
 
 // rows that hold an entry: what lies behind them is read by nobody and holds zeros
 __device__ __forceinline__ int32_t live_rows(const int32_t* live, int64_t n) {
@@ -50,7 +27,7 @@ template <int V>
 __global__ void __launch_bounds__(256)
 permute_kernel(const unsigned char* __restrict__ src, int64_t src_stride, const int32_t* __restrict__ row_of,
                const int32_t* __restrict__ live, int64_t T, int k, int vecs, int segs, unsigned char* __restrict__ dst) {
-  using Vec = typename VecOf<V>::type;
+  using Vec = Raw<V>;
   constexpr int U = 4;
   const int lane = threadIdx.x & 31;
   const int64_t n = T * k, items = T * segs, nwarps = (int64_t)gridDim.x * 8;
@@ -86,19 +63,19 @@ __global__ void __launch_bounds__(256)
 unpermute_kernel(const T* __restrict__ rows, int64_t rows_stride, const int32_t* __restrict__ row_of,
                  const int32_t* __restrict__ live, const float* __restrict__ weights, int64_t tokens, int k, int vecs, int segs,
                  T* __restrict__ out) {
-  using P = Pack<T, V>;
-  constexpr int J = 8 / U;
+  using P = Raw<V>;
+  constexpr int N = V / (int)sizeof(T), J = 8 / U;
   const int lane = threadIdx.x & 31;
   const int64_t n = tokens * k, items = tokens * segs, nwarps = (int64_t)gridDim.x * 8;
   const int32_t n_live = live_rows(live, n);
   for (int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); item < items; item += nwarps) {
     const int64_t t = item / segs;
     const int v0 = (int)(item - t * segs) * (32 * U) + lane;
-    float acc[U][P::N];
+    float acc[U][N];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int i = 0; i < P::N; ++i) acc[u][i] = 0.f;
+      for (int i = 0; i < N; ++i) acc[u][i] = 0.f;
     for (int j0 = 0; j0 < k; j0 += J) {
       int32_t mine = -1;
       float w = 1.f;
@@ -122,21 +99,18 @@ unpermute_kernel(const T* __restrict__ rows, int64_t rows_stride, const int32_t*
         const float wj = __shfl_sync(0xFFFFFFFFu, w, j);
         if (r < 0) continue;
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+          float x[N];
+          unpack<T, V>(p[j][u], x);
 #pragma unroll
-          for (int i = 0; i < P::N; ++i) acc[u][i] = weights ? fmaf(wj, to_f32(p[j][u].e[i]), acc[u][i]) : acc[u][i] + to_f32(p[j][u].e[i]);
+          for (int i = 0; i < N; ++i) acc[u][i] = fmaf(wj, x[i], acc[u][i]);      // by 1 where there are no weights: the sum itself
+        }
       }
     }
     P* d = reinterpret_cast<P*>(out) + t * vecs;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (v0 + 32 * u < vecs) {
-        P o;
-#pragma unroll
-        for (int i = 0; i < P::N; ++i) from_f32(acc[u][i], &o.e[i]);
-        d[v0 + 32 * u] = o;
-      }
-    }
+    for (int u = 0; u < U; ++u)
+      if (v0 + 32 * u < vecs) d[v0 + 32 * u] = pack<T, V>(acc[u]);
   }
 }
 
@@ -147,8 +121,8 @@ __global__ void __launch_bounds__(256)
 unpermute_grad_kernel(const T* __restrict__ gy, int64_t gy_stride, const T* __restrict__ rows, int64_t rows_stride,
                       const int32_t* __restrict__ row_of, const int32_t* __restrict__ live, const float* __restrict__ weights,
                       int64_t tokens, int k, int vecs, T* __restrict__ g_rows, float* __restrict__ g_w) {
-  using P = Pack<T, V>;
-  constexpr int J = 8;
+  using P = Raw<V>;
+  constexpr int N = V / (int)sizeof(T), J = 8;
   __shared__ float part[8][J];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
   const int runs = (k + J - 1) / J;
@@ -168,7 +142,8 @@ unpermute_grad_kernel(const T* __restrict__ gy, int64_t gy_stride, const T* __re
     }
     const P* g = reinterpret_cast<const P*>(gy + t * gy_stride);
     for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
-      const P gv = g[v];
+      float gf[N];
+      unpack<T, V>(g[v], gf);
       P p[J];
       if (g_w) {
 #pragma unroll
@@ -180,14 +155,16 @@ unpermute_grad_kernel(const T* __restrict__ gy, int64_t gy_stride, const T* __re
         if (r[j] < 0) continue;
         const bool has = r[j] < n_live;
         if (g_w && has) {
+          float x[N];
+          unpack<T, V>(p[j], x);
 #pragma unroll
-          for (int i = 0; i < P::N; ++i) dot[j] = fmaf(to_f32(p[j].e[i]), to_f32(gv.e[i]), dot[j]);
+          for (int i = 0; i < N; ++i) dot[j] = fmaf(x[i], gf[i], dot[j]);
         }
         if (g_rows) {
-          P o;
+          float o[N];
 #pragma unroll
-          for (int i = 0; i < P::N; ++i) from_f32(has ? w[j] * to_f32(gv.e[i]) : 0.f, &o.e[i]);
-          reinterpret_cast<P*>(g_rows)[(int64_t)r[j] * vecs + v] = o;
+          for (int i = 0; i < N; ++i) o[i] = has ? w[j] * gf[i] : 0.f;
+          reinterpret_cast<P*>(g_rows)[(int64_t)r[j] * vecs + v] = pack<T, V>(o);
         }
       }
     }
@@ -210,13 +187,6 @@ unpermute_grad_kernel(const T* __restrict__ gy, int64_t gy_stride, const T* __re
 }
 
 static int elem_bytes(int dtype) { return dtype == MOE_DTYPE_F32 ? 4 : 2; }
-
-// widest access that every row of these addresses and strides allows, in bytes (16, 8, 4 or narrower)
-static int vec_bytes(uintptr_t all) {
-  int v = 16;
-  while (v > 1 && (all & (uintptr_t)(v - 1))) v >>= 1;
-  return v;
-}
 
 static unsigned grid_for(int64_t items, int64_t per_cta, int64_t cap) {
   int64_t b = ceil_div64(items, per_cta);
