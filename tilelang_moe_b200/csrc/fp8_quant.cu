@@ -37,8 +37,28 @@ __device__ __forceinline__ Raw<N> quantize(const float* x, float inv) {
     return o;
   }
 }
-// |x| as bits: ordered like the magnitudes, every NaN above infinity
-__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+// max(m, |x|), NaN where either is one
+__device__ __forceinline__ float max_magnitude(float m, float x) {
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(x)));
+  return m;
+}
+// The largest of a group's magnitudes is the largest of their bits: no sign, every NaN above infinity.
+__device__ __forceinline__ float group_top(uint32_t bits) { return __uint_as_float(max(bits, TINY_BITS)); }
+
+// 448 / top and top / 448, each from an approximate quotient and its remainder in one fma (Markstein, IBM J. Res. Dev. 34, 1990);
+// an infinite top has no remainder, and the first quotients, 0 and infinity, stand.  The checked divisions cost as much as
+// the rest of a group: 8192 x 7168 bf16 38.5 -> 36.0 us with both and the maximum by max.NaN.
+__device__ __forceinline__ float inverse_of(float top) {
+  float y;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(top));
+  const float q = TOP * y, rem = fmaf(-top, q, TOP);
+  return fabsf(rem) >= 0.f ? fmaf(rem, y, q) : q;
+}
+__device__ __forceinline__ float scale_of(float top) {
+  constexpr float r = 1.0f / TOP;
+  const float q = top * r, rem = fmaf(-TOP, q, top);
+  return fabsf(rem) >= 0.f ? fmaf(rem, r, q) : q;
+}
 
 struct RowParams {
   const void* x;         // or the gate
@@ -51,13 +71,15 @@ struct RowParams {
   float* scale;
 };
 
-// Groups that a lane has in flight: 64 bytes of loads where a group is one vector per lane, all of the group otherwise.
+// Two vectors of a group per lane, so that what a group costs beside its elements (the steps to its maximum, the quotients,
+// its number) is shared by as many of them: 8192 x 7168 bf16 36.0 -> 30.1 us.  Four vectors of loads in flight per lane, eight
+// where they are narrow (rows of odd widths and strides); twice as many were slower (49 us).
 template <class T, int V, bool SWIGLU>
 struct RowShape {
   static constexpr int N = V / (int)sizeof(T);                  // elements of a vector
-  static constexpr int L = G / N < 32 ? G / N : 32;             // lanes of a group
+  static constexpr int L = V == 16 ? G / (2 * N) : 32;          // lanes of a group
   static constexpr int I = G / (N * L);                         // vectors of a lane and group
-  static constexpr int U = I > 1 ? 1 : (SWIGLU ? 2 : 4);
+  static constexpr int U = (V == 16 ? 4 : 8) / I / (SWIGLU ? 2 : 1);   // groups
   static constexpr int PER_WARP = U * (32 / L);                 // groups of a warp
 };
 
@@ -93,7 +115,7 @@ quantize_rows_kernel(const RowParams p) {
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     float x[I][N];
-    uint32_t m = 0;
+    float m = 0.f;
 #pragma unroll
     for (int i = 0; i < I; ++i) {
       unpack<T, V>(a[u][i], x[i]);
@@ -103,15 +125,20 @@ quantize_rows_kernel(const RowParams p) {
 #pragma unroll
         for (int j = 0; j < N; ++j) x[i][j] = silu_mul(x[i][j], y[j]);
       }
-      uint32_t mine = 0;
+      if (col[u] + i * L * N < p.K) {
 #pragma unroll
-      for (int j = 0; j < N; ++j) mine = max(mine, magnitude(x[i][j]));
-      if (col[u] + i * L * N < p.K) m = max(m, mine);
+        for (int j = 0; j < N; ++j) m = max_magnitude(m, x[i][j]);
+      }
     }
+    uint32_t bits = __float_as_uint(m);
+    if (L == 32) {
+      bits = __reduce_max_sync(0xFFFFFFFFu, bits);
+    } else {
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    const float top = __uint_as_float(max(m, TINY_BITS));
-    const float inv = TOP / top;
+      for (int o = L / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(0xFFFFFFFFu, bits, o));
+    }
+    const float top = group_top(bits);
+    const float inv = inverse_of(top);
     uint8_t* q = p.q + (int64_t)row[u] * p.K;
 #pragma unroll
     for (int i = 0; i < I; ++i) {
@@ -119,7 +146,7 @@ quantize_rows_kernel(const RowParams p) {
       if (c < p.K) *reinterpret_cast<Raw<N>*>(q + c) = quantize<N>(x[i], inv);
     }
     const uint32_t g = first + u * (32 / L);
-    if (in == 0 && g < p.groups) p.scale[g] = top / TOP;
+    if (in == 0 && g < p.groups) p.scale[g] = scale_of(top);
   }
 }
 
@@ -146,22 +173,21 @@ quantize_blocks_kernel(const T* __restrict__ w, int64_t rows, int K, int row_blo
     const int r = r0 + i * STEP;
     if (r < left && col < K) v[i] = *reinterpret_cast<const P*>(w + base + (int64_t)r * K);
   }
-  uint32_t m = 0;
+  float mine = 0.f;
 #pragma unroll
   for (int i = 0; i < I; ++i)
     if (r0 + i * STEP < left && col < K) {
       float x[N];
       unpack<T, V>(v[i], x);
 #pragma unroll
-      for (int j = 0; j < N; ++j) m = max(m, magnitude(x[j]));
+      for (int j = 0; j < N; ++j) mine = max_magnitude(mine, x[j]);
     }
-  m = __reduce_max_sync(0xFFFFFFFFu, m);
+  uint32_t m = __reduce_max_sync(0xFFFFFFFFu, __float_as_uint(mine));
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = max(m, part[i]);
-  const float top = __uint_as_float(max(m, TINY_BITS));
-  const float inv = TOP / top;
+  const float top = group_top(m), inv = inverse_of(top);
 #pragma unroll
   for (int i = 0; i < I; ++i) {
     const int r = r0 + i * STEP;
@@ -171,7 +197,7 @@ quantize_blocks_kernel(const T* __restrict__ w, int64_t rows, int K, int row_blo
       *reinterpret_cast<Raw<N>*>(q + base + (int64_t)r * K) = quantize<N>(x, inv);
     }
   }
-  if (threadIdx.x == 0) scale[blk] = top / TOP;
+  if (threadIdx.x == 0) scale[blk] = scale_of(top);
 }
 
 template <class T, int V, bool SWIGLU>

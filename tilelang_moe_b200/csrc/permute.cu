@@ -21,14 +21,15 @@ __device__ __forceinline__ int32_t live_rows(const int32_t* live, int64_t n) {
   return v < 0 ? 0 : ((int64_t)v > n ? (int32_t)n : v);
 }
 
-// One warp per token and segment of 32 * U vectors: the segment stays in registers while the k places are written.  U = 4
+// One warp per token and segment of 32 * U vectors: the segment stays in registers while the k places are written.  U
 // independent loads per lane, then k * U independent stores.
+template <int V> constexpr int permute_unroll() { return V >= 8 ? 4 : 8; }
 template <int V>
 __global__ void __launch_bounds__(256)
 permute_kernel(const unsigned char* __restrict__ src, int64_t src_stride, const int32_t* __restrict__ row_of,
                const int32_t* __restrict__ live, int64_t T, int k, int vecs, int segs, unsigned char* __restrict__ dst) {
   using Vec = Raw<V>;
-  constexpr int U = 4;
+  constexpr int U = permute_unroll<V>();
   const int lane = threadIdx.x & 31;
   const int64_t n = T * k, items = T * segs, nwarps = (int64_t)gridDim.x * 8;
   const int32_t n_live = live_rows(live, n);
@@ -56,61 +57,66 @@ permute_kernel(const unsigned char* __restrict__ src, int64_t src_stride, const 
   }
 }
 
-// One warp per token and segment of 32 * U vectors: the rows of eight slots are in flight before the first is added, and
-// they are added in slot order, in fp32, with one rounding at the end.
-template <class T, int V, int U>
+// One CTA per token: its rows' numbers and weights stay in registers (k <= 8, ONE) while the threads walk over the width.
+// The eight rows' pieces are in flight before the first is added, U of them each where vectors are narrow; they are added in
+// slot order, in fp32, with one rounding at the end.
+template <class T, int V, bool ONE>
 __global__ void __launch_bounds__(256)
 unpermute_kernel(const T* __restrict__ rows, int64_t rows_stride, const int32_t* __restrict__ row_of,
-                 const int32_t* __restrict__ live, const float* __restrict__ weights, int64_t tokens, int k, int vecs, int segs,
+                 const int32_t* __restrict__ live, const float* __restrict__ weights, int64_t tokens, int k, int vecs,
                  T* __restrict__ out) {
   using P = Raw<V>;
-  constexpr int N = V / (int)sizeof(T), J = 8 / U;
-  const int lane = threadIdx.x & 31;
-  const int64_t n = tokens * k, items = tokens * segs, nwarps = (int64_t)gridDim.x * 8;
-  const int32_t n_live = live_rows(live, n);
-  for (int64_t item = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); item < items; item += nwarps) {
-    const int64_t t = item / segs;
-    const int v0 = (int)(item - t * segs) * (32 * U) + lane;
-    float acc[U][N];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int i = 0; i < N; ++i) acc[u][i] = 0.f;
-    for (int j0 = 0; j0 < k; j0 += J) {
-      int32_t mine = -1;
-      float w = 1.f;
-      if (lane < J && j0 + lane < k) {
-        mine = row_of[t * k + j0 + lane];
-        if (weights) w = weights[t * k + j0 + lane];
-      }
-      if (mine >= n_live) mine = -1;
-      P p[J][U];
+  constexpr int N = V / (int)sizeof(T), J = 8, U = V == 16 ? 1 : (V == 8 ? 2 : 4);
+  const int32_t n_live = live_rows(live, tokens * k);
+  for (int64_t t = blockIdx.x; t < tokens; t += gridDim.x) {
+    int32_t r[J];
+    float w[J];
+    auto look_up = [&](int j0) {
 #pragma unroll
       for (int j = 0; j < J; ++j) {
-        const int32_t r = __shfl_sync(0xFFFFFFFFu, mine, j);
-        const P* s = reinterpret_cast<const P*>(rows + (int64_t)r * rows_stride);
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-          if (r >= 0 && v0 + 32 * u < vecs) p[j][u] = s[v0 + 32 * u];
-      }
-#pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int32_t r = __shfl_sync(0xFFFFFFFFu, mine, j);
-        const float wj = __shfl_sync(0xFFFFFFFFu, w, j);
-        if (r < 0) continue;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          float x[N];
-          unpack<T, V>(p[j][u], x);
-#pragma unroll
-          for (int i = 0; i < N; ++i) acc[u][i] = fmaf(wj, x[i], acc[u][i]);      // by 1 where there are no weights: the sum itself
+        r[j] = -1;
+        w[j] = 1.f;
+        if (j0 + j < k) {
+          r[j] = row_of[t * k + j0 + j];
+          if (weights) w[j] = weights[t * k + j0 + j];
+          if (r[j] >= n_live) r[j] = -1;
         }
       }
-    }
+    };
+    if (ONE) look_up(0);
     P* d = reinterpret_cast<P*>(out) + t * vecs;
+    for (int v0 = threadIdx.x; v0 < vecs; v0 += blockDim.x * U) {
+      float acc[U][N];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (v0 + 32 * u < vecs) d[v0 + 32 * u] = pack<T, V>(acc[u]);
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[u][i] = 0.f;
+      for (int j0 = 0; j0 < (ONE ? 1 : k); j0 += J) {
+        if (!ONE) look_up(j0);
+        P p[J][U];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          const P* s = reinterpret_cast<const P*>(rows + (int64_t)r[j] * rows_stride);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (r[j] >= 0 && v0 + u * (int)blockDim.x < vecs) p[j][u] = s[v0 + u * blockDim.x];
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (r[j] < 0) continue;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            float x[N];
+            unpack<T, V>(p[j][u], x);
+#pragma unroll
+            for (int i = 0; i < N; ++i) acc[u][i] = fmaf(w[j], x[i], acc[u][i]);      // by 1 where there are no weights: the sum itself
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (v0 + u * (int)blockDim.x < vecs) d[v0 + u * blockDim.x] = pack<T, V>(acc[u]);
+    }
   }
 }
 
@@ -122,7 +128,7 @@ unpermute_grad_kernel(const T* __restrict__ gy, int64_t gy_stride, const T* __re
                       const int32_t* __restrict__ row_of, const int32_t* __restrict__ live, const float* __restrict__ weights,
                       int64_t tokens, int k, int vecs, T* __restrict__ g_rows, float* __restrict__ g_w) {
   using P = Raw<V>;
-  constexpr int N = V / (int)sizeof(T), J = 8;
+  constexpr int N = V / (int)sizeof(T), J = 8, U = V == 16 ? 1 : (V == 8 ? 2 : 4);
   __shared__ float part[8][J];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nwarps = blockDim.x >> 5;
   const int runs = (k + J - 1) / J;
@@ -141,30 +147,42 @@ unpermute_grad_kernel(const T* __restrict__ gy, int64_t gy_stride, const T* __re
       dot[j] = 0.f;
     }
     const P* g = reinterpret_cast<const P*>(gy + t * gy_stride);
-    for (int v = threadIdx.x; v < vecs; v += blockDim.x) {
-      float gf[N];
-      unpack<T, V>(g[v], gf);
-      P p[J];
+    for (int v0 = threadIdx.x; v0 < vecs; v0 += blockDim.x * U) {
+      P graw[U], p[J][U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (v0 + u * (int)blockDim.x < vecs) graw[u] = g[v0 + u * blockDim.x];
       if (g_w) {
 #pragma unroll
-        for (int j = 0; j < J; ++j)
-          if (r[j] >= 0 && r[j] < n_live) p[j] = reinterpret_cast<const P*>(rows + (int64_t)r[j] * rows_stride)[v];
+        for (int j = 0; j < J; ++j) {
+          const P* s = reinterpret_cast<const P*>(rows + (int64_t)r[j] * rows_stride);
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (r[j] >= 0 && r[j] < n_live && v0 + u * (int)blockDim.x < vecs) p[j][u] = s[v0 + u * blockDim.x];
+        }
       }
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        if (r[j] < 0) continue;
-        const bool has = r[j] < n_live;
-        if (g_w && has) {
-          float x[N];
-          unpack<T, V>(p[j], x);
+      for (int u = 0; u < U; ++u) {
+        const int v = v0 + u * blockDim.x;
+        if (v >= vecs) break;
+        float gf[N];
+        unpack<T, V>(graw[u], gf);
 #pragma unroll
-          for (int i = 0; i < N; ++i) dot[j] = fmaf(x[i], gf[i], dot[j]);
-        }
-        if (g_rows) {
-          float o[N];
+        for (int j = 0; j < J; ++j) {
+          if (r[j] < 0) continue;
+          const bool has = r[j] < n_live;
+          if (g_w && has) {
+            float x[N];
+            unpack<T, V>(p[j][u], x);
 #pragma unroll
-          for (int i = 0; i < N; ++i) o[i] = has ? w[j] * gf[i] : 0.f;
-          reinterpret_cast<P*>(g_rows)[(int64_t)r[j] * vecs + v] = pack<T, V>(o);
+            for (int i = 0; i < N; ++i) dot[j] = fmaf(x[i], gf[i], dot[j]);
+          }
+          if (g_rows) {
+            float o[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) o[i] = has ? w[j] * gf[i] : 0.f;
+            reinterpret_cast<P*>(g_rows)[(int64_t)r[j] * vecs + v] = pack<T, V>(o);
+          }
         }
       }
     }
@@ -184,6 +202,12 @@ unpermute_grad_kernel(const T* __restrict__ gy, int64_t gy_stride, const T* __re
       __syncthreads();
     }
   }
+}
+
+// threads of a CTA that walks over `vecs` vectors of V bytes
+static unsigned threads_for(int vecs, int V) {
+  const int work = (vecs + (V == 16 ? 0 : (V == 8 ? 1 : 3))) / (V == 16 ? 1 : (V == 8 ? 2 : 4));
+  return work >= 256 ? 256u : (unsigned)((work + 31) / 32 * 32);
 }
 
 static int elem_bytes(int dtype) { return dtype == MOE_DTYPE_F32 ? 4 : 2; }
@@ -220,7 +244,7 @@ extern "C" int moe_permute(const void* src, int64_t src_stride, int64_t row_byte
   int rc = current_device_info(&dev);
   if (rc) return rc;
   const int V = vec_bytes(reinterpret_cast<uintptr_t>(src) | reinterpret_cast<uintptr_t>(dst) | (uintptr_t)src_stride | (uintptr_t)row_bytes);
-  const int vecs = (int)(row_bytes / V), segs = (vecs + 127) / 128;
+  const int vecs = (int)(row_bytes / V), segs = (vecs + (V >= 8 ? 127 : 255)) / (V >= 8 ? 128 : 256);
   const unsigned grid = grid_for(T * segs, 8, (int64_t)dev.sm_count * 8);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const unsigned char* s = reinterpret_cast<const unsigned char*>(src);
@@ -243,10 +267,11 @@ static void launch_unpermute(const void* rows, int64_t stride, const int32_t* ro
                              int k, int64_t H, void* out, int sms, cudaStream_t st) {
   using namespace moe::perm;
   const int vecs = (int)(H * sizeof(T) / V);
-  constexpr int U = V == 16 ? 1 : 4;       // narrow vectors: more of them per lane
-  const int segs = (vecs + 32 * U - 1) / (32 * U);
-  unpermute_kernel<T, V, U><<<grid_for(tokens * segs, 8, (int64_t)sms * 8), 256, 0, st>>>(
-      reinterpret_cast<const T*>(rows), stride, row_of, live, w, tokens, k, vecs, segs, reinterpret_cast<T*>(out));
+  const unsigned grid = grid_for(tokens, 1, (int64_t)sms * 8), threads = threads_for(vecs, V);
+  const T* r = reinterpret_cast<const T*>(rows);
+  T* o = reinterpret_cast<T*>(out);
+  if (k <= 8) unpermute_kernel<T, V, true><<<grid, threads, 0, st>>>(r, stride, row_of, live, w, tokens, k, vecs, o);
+  else unpermute_kernel<T, V, false><<<grid, threads, 0, st>>>(r, stride, row_of, live, w, tokens, k, vecs, o);
 }
 
 extern "C" int moe_unpermute(const void* rows, int64_t rows_stride, const int32_t* row_of, const int32_t* live, const float* weights,
@@ -282,7 +307,7 @@ static void launch_unpermute_grad(const void* gy, int64_t gy_stride, const void*
                                   int sms, cudaStream_t st) {
   using namespace moe::perm;
   const int vecs = (int)(H * sizeof(T) / V);
-  const unsigned threads = vecs >= 256 ? 256u : (unsigned)((vecs + 31) / 32 * 32);
+  const unsigned threads = threads_for(vecs, V);
   const int64_t items = tokens * ((k + 7) / 8);
   unpermute_grad_kernel<T, V><<<grid_for(items, 1, (int64_t)sms * 8), threads, 0, st>>>(
       reinterpret_cast<const T*>(gy), gy_stride, reinterpret_cast<const T*>(rows), rows_stride, row_of, live, w, tokens, k, vecs,
