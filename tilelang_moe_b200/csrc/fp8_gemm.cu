@@ -30,6 +30,8 @@ constexpr int NUM_THREADS = 320;
 constexpr int EPI_WARPS = 8;
 constexpr int MAX_E = 1024;
 
+constexpr int MAX_SPLIT = 8;            // CTAs of a cluster that share a tile's k-blocks
+
 template <int BN>
 struct Cfg {
   static constexpr int A_BYTES = BM * BK;
@@ -42,6 +44,8 @@ struct Cfg {
   static constexpr int TABLE_OFFSET = (SLOT_OFFSET + 16 + 15) & ~15;
   static constexpr int SMEM_BYTES = TABLE_OFFSET + 2 * (MAX_E + 1) * 4 + 1024;    // + alignment slack
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
+  static constexpr int PART_PITCH = BN + 4;                     // floats per row of a partial tile, which lies where the stages were
+  static_assert(BM * PART_PITCH * 4 <= BAR_OFFSET, "a partial tile fits the stages");
 };
 
 struct Params {
@@ -56,6 +60,7 @@ struct Params {
   int out;                       // MOE_DTYPE_*
   int vec_store;                 // rows of Y take 16-byte stores
   int zero_tail;                 // rows of no group are set to zero
+  int a_box_rows;                // rows of A that a stage brings (fewer than a tile's where A has fewer)
   int32_t* status;
 };
 
@@ -183,6 +188,30 @@ __device__ __forceinline__ void store_row(const Params& p, int64_t row, int col0
   }
 }
 
+__device__ __forceinline__ void store_four(const Params& p, int64_t row, int col, float4 v) {
+  unsigned char* y = reinterpret_cast<unsigned char*>(p.Y) + (row * p.ldy + col) * (p.out == MOE_DTYPE_F32 ? 4 : 2);
+  if (p.vec_store) {
+    if (col >= p.N) return;                     // N is a multiple of four or eight then
+    if (p.out == MOE_DTYPE_F32) *reinterpret_cast<float4*>(y) = v;
+    else *reinterpret_cast<uint2*>(y) = make_uint2(pack16(pair_of(v.x, v.y), p.out), pack16(pair_of(v.z, v.w), p.out));
+  } else {
+    const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (col + j < p.N) {
+        if (p.out == MOE_DTYPE_F32) reinterpret_cast<float*>(y)[j] = e[j];
+        else reinterpret_cast<uint16_t*>(y)[j] = one16(e[j], p.out);
+      }
+    }
+  }
+}
+// four floats of a CTA of this cluster (an address from map_to_cta)
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+
 // rows of no group, before the first one and behind the last, set to zero; warps w of n
 __device__ __forceinline__ void zero_rows(const Params& p, int64_t ahead, int64_t behind, int64_t w, int64_t n, int lane) {
   for (int64_t i = w; i < ahead + p.rows - behind; i += n) {
@@ -195,7 +224,9 @@ __device__ __forceinline__ void zero_rows(const Params& p, int64_t ahead, int64_
   }
 }
 
-template <int BN>
+// SPLIT: the CTAs of a cluster take a run of the k-blocks each, of one tile per cluster; what they have accumulated meets in
+// shared memory and is added in the order of the CTAs.  For products of few tiles, which would leave most SMs without one.
+template <int BN, bool SPLIT>
 __global__ void __launch_bounds__(NUM_THREADS, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
   using C = Cfg<BN>;
@@ -214,7 +245,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
   const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
   const uint32_t tfull0 = smem_u32(bars + 2 * STAGES), tempty0 = smem_u32(bars + 2 * STAGES + 2);
   const uint32_t drain_bar = smem_u32(bars + 2 * STAGES + 4);
-  const int E = p.E, NT = p.n_tiles, NKB = p.k_blocks;
+  const int E = p.E, NT = p.n_tiles;
+  const int S = SPLIT ? (int)cluster_nctarank() : 1, rank = SPLIT ? (int)cluster_ctarank() : 0;
+  const int first_tile = SPLIT ? (int)blockIdx.x / S : (int)blockIdx.x, tile_step = SPLIT ? 1 << 30 : (int)gridDim.x;
+  const int kb0 = SPLIT ? (int)((int64_t)p.k_blocks * rank / S) : 0;                      // this CTA's k-blocks
+  const int kb1 = SPLIT ? (int)((int64_t)p.k_blocks * (rank + 1) / S) : p.k_blocks;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) { mbar_init(full0 + 8 * s, 1); mbar_init(empty0 + 8 * s, 1); }
@@ -244,14 +279,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     int stage = 0;
     uint32_t phase = 0, issued = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
+    for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
       const Tile t = decode_tile(tile, tstart, offs, E, NT);
-      for (int kb = 0; kb < NKB; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, abort_flag, p.status, 31)) { ok = false; break; }
         if (lane == 0) {
           const uint32_t full = full0 + 8 * stage;
           const uint32_t sa = smem_u32(smem + stage * C::STAGE_BYTES);
-          mbar_arrive_expect_tx(full, C::STAGE_BYTES);
+          mbar_arrive_expect_tx(full, p.a_box_rows * BK + C::B_BYTES);
           tma_load_2d(sa, &tmA, full, kb * BK, t.row0);
           tma_load_3d(sa + C::A_BYTES, &tmB, full, kb * BK, t.n_tile * BN, t.e);
         }
@@ -275,8 +310,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
-        for (int kb = 0; kb < NKB; ++kb) {
+      for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
+        for (int kb = kb0; kb < kb1; ++kb) {
           if (!mbar_wait(full0 + 8 * stage, phase, abort_flag, p.status, 33)) { ok = false; break; }
           if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, p.status, 32)) { ok = false; break; }
           tc_fence_after();
@@ -305,20 +340,20 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     int buf = 0;
     uint32_t buf_phase = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; ok && tile < total_tiles; tile += gridDim.x) {
+    for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
       const Tile t = decode_tile(tile, tstart, offs, E, NT);
       const int row = t.row0 + q * 32 + lane, col0 = t.n_tile * BN + half * COLS;
       const bool row_ok = row < t.row_end;
-      const float* sa = p.sa + (row_ok ? (int64_t)row * p.sa_row : 0);
+      const float* sa = p.sa + (row_ok ? (int64_t)row * p.sa_row : 0) + kb0 * p.sa_k;
       // columns behind N have no scale block of their own: the last one stands in, nothing of them is stored
-      const float* sb = p.sb + ((int64_t)t.e * p.n_blocks + min(col0 / 128, p.n_blocks - 1)) * NKB;
+      const float* sb = p.sb + ((int64_t)t.e * p.n_blocks + min(col0 / 128, p.n_blocks - 1)) * p.k_blocks + kb0;
       f32x2 acc[COLS / 2];
 #pragma unroll
       for (int j = 0; j < COLS / 2; ++j) acc[j] = 0ull;
       float s_next = sa[0] * sb[0];
-      for (int kb = 0; kb < NKB; ++kb) {
+      for (int kb = kb0; kb < kb1; ++kb) {
         const float s = s_next;
-        if (kb + 1 < NKB) s_next = sa[(kb + 1) * p.sa_k] * sb[kb + 1];
+        if (kb + 1 < kb1) s_next = sa[(kb + 1 - kb0) * p.sa_k] * sb[kb + 1 - kb0];
         if (!mbar_wait(tfull0 + 8 * buf, buf_phase, abort_flag, p.status, 34)) { ok = false; break; }
         tc_fence_after();
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + half * COLS);
@@ -335,9 +370,40 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         if (lane == 0) mbar_arrive(tempty0 + 8 * buf);
         if (++buf == 2) { buf = 0; buf_phase ^= 1; }
       }
-      if (ok && row_ok) store_row<COLS>(p, row, col0, acc);
+      if (SPLIT) {
+        // every stage has been consumed by the time the last accumulator was ready: the partial tile may take their place
+        float* mine = reinterpret_cast<float*>(smem) + (q * 32 + lane) * C::PART_PITCH + half * COLS;
+#pragma unroll
+        for (int j = 0; j < COLS / 2; j += 2)
+          if (row_ok) *reinterpret_cast<ulonglong2*>(mine + 2 * j) = make_ulonglong2(acc[j], acc[j + 1]);
+      } else if (ok && row_ok) {
+        store_row<COLS>(p, row, col0, acc);
+      }
     }
     if (p.zero_tail) zero_rows(p, offs[0], offs[E], (int64_t)blockIdx.x * EPI_WARPS + (warp - 2), (int64_t)gridDim.x * EPI_WARPS, lane);
+  }
+
+  if (SPLIT) {
+    __syncthreads();
+    cluster_barrier();
+    if (first_tile < total_tiles && threadIdx.x < 256 && !*abort_flag) {
+      const Tile t = decode_tile(first_tile, tstart, offs, E, NT);
+      const int live = min(BM, t.row_end - t.row0);
+      for (int i = rank * 256 + threadIdx.x; i < live * (BN / 4); i += S * 256) {
+        const int r = i / (BN / 4), c = (i - r * (BN / 4)) * 4;
+        const uint32_t at = smem_u32(smem) + (uint32_t)(r * C::PART_PITCH + c) * 4;
+        float4 v[MAX_SPLIT];
+#pragma unroll
+        for (int s = 0; s < MAX_SPLIT; ++s)
+          if (s < S) v[s] = ld_cluster(map_to_cta(at, s));
+        float4 sum = v[0];
+#pragma unroll
+        for (int s = 1; s < MAX_SPLIT; ++s)
+          if (s < S) { sum.x += v[s].x; sum.y += v[s].y; sum.z += v[s].z; sum.w += v[s].w; }
+        store_four(p, t.row0 + r, t.n_tile * BN + c, sum);
+      }
+    }
+    cluster_barrier();        // nobody leaves while its partial tile is still read
   }
 
   // ---- teardown
@@ -367,21 +433,33 @@ static int make_tmap8(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1
   return MOE_OK;
 }
 
-template <int BN>
-static int launch(const void* A, int64_t lda, const void* B, Params p, int sms, cudaStream_t st) {
+// split: CTAs per cluster, or 1
+template <int BN, bool SPLIT>
+static int launch(const void* A, int64_t lda, const void* B, Params p, int64_t tiles, int split, int sms, cudaStream_t st) {
   using C = Cfg<BN>;
+  auto kernel = fp8_gemm_kernel<BN, SPLIT>;
   static std::atomic<bool> attr_set[64];
-  int rc = allow_dynamic_smem(fp8_gemm_kernel<BN>, C::SMEM_BYTES, attr_set);
+  int rc = allow_dynamic_smem(kernel, C::SMEM_BYTES, attr_set);
   if (rc) return rc;
   p.n_tiles = (p.N + BN - 1) / BN;
-  const int64_t bound = ((int64_t)p.rows / BM + p.E) * p.n_tiles;
-  if (bound > 0x7FFFFFFFll) return fail(MOE_ERR_UNSUPPORTED, "fp8_gemm: too many tiles");
   CUtensorMap tA, tB;
-  rc = make_tmap8(&tA, A, (uint64_t)p.K, (uint64_t)p.rows, 0, (uint64_t)lda, (uint32_t)BM);
+  rc = make_tmap8(&tA, A, (uint64_t)p.K, (uint64_t)p.rows, 0, (uint64_t)lda, (uint32_t)p.a_box_rows);
   if (rc) return rc;
   rc = make_tmap8(&tB, B, (uint64_t)p.K, (uint64_t)p.N, (uint64_t)p.E, (uint64_t)p.K, (uint32_t)BN);
   if (rc) return rc;
-  MOE_LAUNCH("fp8_gemm_kernel", fp8_gemm_kernel<BN>, (unsigned)(bound < sms ? bound : sms), NUM_THREADS, C::SMEM_BYTES, st, false, tA, tB, p);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(SPLIT ? tiles * split : (tiles < sms ? tiles : sms)), 1, 1);
+  cfg.blockDim = dim3(NUM_THREADS, 1, 1);
+  cfg.dynamicSmemBytes = C::SMEM_BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = SPLIT ? 1 : 0;
+  MOE_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, tA, tB, p));
   return MOE_OK;
 }
 
@@ -417,5 +495,16 @@ extern "C" int moe_fp8_gemm(const void* A, int64_t lda, const float* a_scale, in
   const int64_t el = out_dtype == MOE_DTYPE_F32 ? 4 : 2;
   p.vec_store = !(reinterpret_cast<uintptr_t>(Y) & 15) && (ldy * el) % 16 == 0 && (N * el) % 16 == 0;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  return launch<256>(A, lda, B, p, dev.sm_count, st);
+  // Tiles of 256 columns where they give every SM one: they bring the least operand traffic per product.  Fewer tiles take
+  // 128 columns, and where even those leave SMs idle, clusters of 2, 4 or 8 CTAs share the k-blocks of a tile (clusters of
+  // 4 and 8 do not fill the GPU: counted as 128 SMs), two k-blocks each at least.
+  const int64_t m_tiles = offsets ? rows / BM + (rows < E ? rows : E) : ceil_div64(rows, BM);
+  const int64_t tiles256 = m_tiles * ceil_div64(N, 256), tiles128 = m_tiles * ceil_div64(N, 128);
+  if (tiles128 > 0x7FFFFFFFll) return fail(MOE_ERR_UNSUPPORTED, "fp8_gemm: too many tiles");
+  p.a_box_rows = rows < BM ? (int)(rows + 7) / 8 * 8 : BM;
+  if (tiles256 >= dev.sm_count) return launch<256, false>(A, lda, B, p, tiles256, 1, dev.sm_count, st);
+  int split = 1;
+  while (split < MAX_SPLIT && p.k_blocks >= 4 * split && tiles128 * split * 2 <= (split == 1 ? dev.sm_count : dev.sm_count * 7 / 8)) split *= 2;
+  if (split > 1) return launch<128, true>(A, lda, B, p, tiles128, split, dev.sm_count, st);
+  return launch<128, false>(A, lda, B, p, tiles128, 1, dev.sm_count, st);
 }

@@ -49,8 +49,8 @@ def fp8_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     ops._need_cuda(x)
     dt = _input_type(x, 1)
     K = x.shape[-1]
-    q = torch.empty(x.shape, dtype=E4M3, device=x.device)
-    scale = torch.empty(*x.shape[:-1], _groups(K), dtype=torch.float32, device=x.device)
+    q = x.new_empty(x.shape, dtype=E4M3)
+    scale = x.new_empty((*x.shape[:-1], _groups(K)), dtype=torch.float32)
     rows = _rows2(x)
     with ops._on(x.device):
         rc = _lib.load().moe_fp8_quantize_rows(ops._ptr(rows), _stride(rows), rows.shape[0], K, dt, ops._ptr(q), ops._ptr(scale),
@@ -68,8 +68,8 @@ def fp8_silu_mul(gate: torch.Tensor, up: torch.Tensor) -> Tuple[torch.Tensor, to
     if up.shape != gate.shape or up.dtype != gate.dtype or up.device != gate.device:
         raise ValueError("gate and up must have one shape and type and be on one device")
     I = gate.shape[-1]
-    q = torch.empty(gate.shape, dtype=E4M3, device=gate.device)
-    scale = torch.empty(*gate.shape[:-1], _groups(I), dtype=torch.float32, device=gate.device)
+    q = gate.new_empty(gate.shape, dtype=E4M3)
+    scale = gate.new_empty((*gate.shape[:-1], _groups(I)), dtype=torch.float32)
     g, u = _rows2(gate), _rows2(up)
     with ops._on(gate.device):
         rc = _lib.load().moe_fp8_silu_mul(ops._ptr(g), _stride(g), ops._ptr(u), _stride(u), g.shape[0], I, dt, ops._ptr(q), ops._ptr(scale),

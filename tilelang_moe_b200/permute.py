@@ -37,6 +37,13 @@ class MoESort:
         if not (self.offsets.device == self.perm.device == self.row_of.device):
             raise ValueError("the tables of a sort must be on one device")
 
+    @classmethod
+    def _of(cls, offsets, perm, row_of, k) -> "MoESort":
+        """Tables that moe_sort has just laid out: as they should be without looking."""
+        s = object.__new__(cls)
+        s.__dict__.update(offsets=offsets, perm=perm, row_of=row_of, k=k)
+        return s
+
     @property
     def n_experts(self) -> int:
         return self.offsets.numel() - 1
@@ -60,8 +67,7 @@ def moe_sort(topk_ids: torch.Tensor, n_experts: int) -> MoESort:
     lib = _lib.load()
     # one allocation: counts [E + 1], offsets [E + 2], perm [n], row_of [n]
     buf = torch.empty(2 * n_experts + 3 + 2 * n, dtype=torch.int32, device=dev)
-    at = n_experts + 1
-    offsets, perm, row_of = buf[at:at + n_experts + 1], buf[at + n_experts + 2:at + n_experts + 2 + n], buf[at + n_experts + 2 + n:]
+    _, offsets, _, perm, row_of = buf.split_with_sizes((n_experts + 1, n_experts + 1, 1, n, n))
     need = lib.moe_sort_workspace(n, n_experts)
     ws = torch.empty(max(need, 4), dtype=torch.uint8, device=dev)
     with ops._on(dev):
@@ -69,7 +75,7 @@ def moe_sort(topk_ids: torch.Tensor, n_experts: int) -> MoESort:
                           ops._ptr(perm), ops._ptr(row_of), ops._ptr(ws), need, ops._stream())
     _lib.check(rc, "moe_sort")
     ops._after(dev)
-    return MoESort(offsets, perm, row_of, ids.shape[1] if ids.dim() == 2 else 1)
+    return MoESort._of(offsets, perm, row_of, ids.shape[1] if ids.dim() == 2 else 1)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -85,7 +91,7 @@ def _permute(x: torch.Tensor, sort: MoESort) -> torch.Tensor:
     x = _rows(x)
     T, H = x.shape
     w = x.element_size()
-    out = torch.empty(T * sort.k, H, dtype=x.dtype, device=x.device)
+    out = x.new_empty((T * sort.k, H))
     with ops._on(x.device):
         rc = _lib.load().moe_permute(ops._ptr(x), _stride(x) * w, H * w, ops._ptr(sort.row_of), ops._ptr(sort.offsets) + 4 * sort.n_experts,
                                      T, sort.k, ops._ptr(out), ops._stream())
@@ -97,7 +103,7 @@ def _permute(x: torch.Tensor, sort: MoESort) -> torch.Tensor:
 def _unpermute(rows: torch.Tensor, sort: MoESort, weights: Optional[torch.Tensor]) -> torch.Tensor:
     rows = _rows(rows)
     T, H = sort.tokens, rows.shape[1]
-    out = torch.empty(T, H, dtype=rows.dtype, device=rows.device)
+    out = rows.new_empty((T, H))
     with ops._on(rows.device):
         rc = _lib.load().moe_unpermute(ops._ptr(rows), _stride(rows), ops._ptr(sort.row_of), ops._ptr(sort.offsets) + 4 * sort.n_experts,
                                        ops._ptr(weights), T, sort.k, H, _DTYPES[rows.dtype], ops._ptr(out), ops._stream())
