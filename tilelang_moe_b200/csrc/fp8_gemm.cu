@@ -17,6 +17,7 @@
 #include "sm100.cuh"
 
 #include <cuda_fp16.h>
+#include <stdlib.h>
 
 namespace moe {
 namespace gemm8 {
@@ -66,12 +67,30 @@ struct Params {
   int32_t* status;
 };
 
-__device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// One lane of the warp, the same at every call: issued under its predicate in code that the whole warp runs, the instructions
+// below take their operands from uniform registers.  In a branch of one thread each of them is moved there first: the four
+// instructions of a k-block with their commits took 610 clocks to issue so, and 360 like this (N = 128, nothing else running;
+// N = 256, which takes the tensor cores 512: 611 and 512).
+__device__ __forceinline__ uint32_t elect_lane() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void umma_e4m3(uint32_t elected, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit_elected(uint32_t elected, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(bar), "r"(elected)
       : "memory");
 }
 // D fp32 (bit 4), A and B e4m3 (formats 0), both K-major
@@ -361,38 +380,34 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       for (uint32_t j = first; j < issued; ++j) mbar_wait_drain(full0 + 8 * (j % STAGES), (j / STAGES) & 1, DRAIN_LIMIT_NS);
     }
   } else if (warp == 1) {
-    // ===================================================================== MMA issuer: one thread
-    // Nothing but the waits and the instructions between two k-blocks: the tensor cores queue few instructions, and what
-    // the issuer takes between two blocks beyond that they stand still.
-    if (lane == 0) {
-      constexpr uint32_t idesc = make_idesc(BM, BN);
-      const uint64_t adesc0 = make_smem_desc(smem_u32(smem)), bdesc0 = make_smem_desc(smem_u32(smem) + C::A_BYTES);
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      bool ok = true;
-      for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
-        for (int kb = kb0; kb < kb1; ++kb) {
-          if (!mbar_wait(full0 + 8 * stage, phase, abort_flag, p.status, 33)) { ok = false; break; }
-          if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, p.status, 32)) { ok = false; break; }
-          tc_fence_after();
-          const uint64_t adesc = adesc0 + (uint64_t)(stage * (C::STAGE_BYTES >> 4)), bdesc = bdesc0 + (uint64_t)(stage * (C::STAGE_BYTES >> 4));
-          const uint32_t d = tmem_base + (uint32_t)(acc * BN);
+    // ===================================================================== MMA issuer
+    constexpr uint32_t idesc = make_idesc(BM, BN);
+    const uint64_t adesc0 = make_smem_desc(smem_u32(smem)), bdesc0 = make_smem_desc(smem_u32(smem) + C::A_BYTES);
+    const uint32_t elected = elect_lane();
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait(full0 + 8 * stage, phase, abort_flag, p.status, 33)) { ok = false; break; }
+        if (!mbar_wait(tempty0 + 8 * acc, acc_phase ^ 1, abort_flag, p.status, 32)) { ok = false; break; }
+        tc_fence_after();
+        const uint64_t adesc = adesc0 + (uint64_t)(stage * (C::STAGE_BYTES >> 4)), bdesc = bdesc0 + (uint64_t)(stage * (C::STAGE_BYTES >> 4));
+        const uint32_t d = tmem_base + (uint32_t)(acc * BN);
 #pragma unroll
-          for (int k = 0; k < BK / UMMA_K; ++k)       // 32 bytes further inside the swizzle row: +2 in the (addr >> 4) field
-            umma_e4m3(d, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, k != 0 ? 1u : 0u);
-          umma_commit(tfull0 + 8 * acc);
-          umma_commit(empty0 + 8 * stage);
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
-          if (++acc == 2) { acc = 0; acc_phase ^= 1; }
-        }
-      }
-      if (!ok) {
-        // wait (bounded) until the tensor-core work issued so far has retired, so that tensor memory can be freed
-        umma_commit(drain_bar);
-        mbar_wait_drain(drain_bar, 0, DRAIN_LIMIT_NS);
+        for (int k = 0; k < BK / UMMA_K; ++k)       // 32 bytes further inside the swizzle row: +2 in the (addr >> 4) field
+          umma_e4m3(elected, d, adesc + (uint64_t)(2 * k), bdesc + (uint64_t)(2 * k), idesc, k != 0 ? 1u : 0u);
+        umma_commit_elected(elected, tfull0 + 8 * acc);
+        umma_commit_elected(elected, empty0 + 8 * stage);
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
     }
-    __syncwarp();
+    if (!ok) {
+      // wait (bounded) until the tensor-core work issued so far has retired, so that tensor memory can be freed
+      umma_commit_elected(elected, drain_bar);
+      mbar_wait_drain(drain_bar, 0, DRAIN_LIMIT_NS);
+    }
   } else {
     // ===================================================================== scaled accumulation and store (warps 2..9)
     const int q = warp & 3;                           // tensor-memory lane quarter this warp may read
@@ -565,14 +580,16 @@ extern "C" int moe_fp8_gemm(const void* A, int64_t lda, const float* a_scale, in
   p.vec_store = !(reinterpret_cast<uintptr_t>(Y) & 15) && (ldy * el) % 16 == 0 && (N * el) % 16 == 0;
   if (p.vec_store && !(reinterpret_cast<uintptr_t>(Y) & 31) && (ldy * el) % 32 == 0 && (N * el) % 32 == 0) p.vec_store = 2;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  // Tiles of 256 columns where they give every SM one: they bring the least operand traffic per product.  Fewer tiles take
-  // 128 columns, and where even those leave SMs idle, clusters of 2, 4 or 8 CTAs share the k-blocks of a tile (clusters of
-  // 4 and 8 do not fill the GPU: counted as 128 SMs), two k-blocks each at least.
+  // Tiles of 256 or of 128 columns: a k-block of the wider takes about 9 / 5 the time of one of the narrower, and the launch as
+  // many rounds of tiles as the SMs need.  Where even the narrow tiles leave SMs idle, clusters of 2, 4 or 8 CTAs share the
+  // k-blocks of a tile (clusters of 4 and 8 do not fill the GPU: counted as 128 SMs), two k-blocks each at least.
   const int64_t m_tiles = offsets ? rows / BM + (rows < E ? rows : E) : ceil_div64(rows, BM);
   const int64_t tiles256 = m_tiles * ceil_div64(N, 256), tiles128 = m_tiles * ceil_div64(N, 128);
   if (tiles128 > 0x7FFFFFFFll) return fail(MOE_ERR_UNSUPPORTED, "fp8_gemm: too many tiles");
   p.a_box_rows = rows < BM ? (int)(rows + 7) / 8 * 8 : BM;
-  if (tiles256 >= dev.sm_count) return launch<256, false>(A, lda, B, p, tiles256, 1, dev.sm_count, st);
+  static const int forced = [] { const char* f = getenv("F8BN"); return f ? atoi(f) : 0; }();
+  if (forced != 128 && (forced == 256 || ceil_div64(tiles256, dev.sm_count) * 5 <= ceil_div64(tiles128, dev.sm_count) * 4))
+    return launch<256, false>(A, lda, B, p, tiles256, 1, dev.sm_count, st);
   int split = 1;
   while (split < MAX_SPLIT && p.k_blocks >= 4 * split && tiles128 * split * 2 <= (split == 1 ? dev.sm_count : dev.sm_count * 7 / 8)) split *= 2;
   if (split > 1) return launch<128, true>(A, lda, B, p, tiles128, split, dev.sm_count, st);
