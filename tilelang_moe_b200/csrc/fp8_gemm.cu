@@ -17,7 +17,6 @@
 #include "sm100.cuh"
 
 #include <cuda_fp16.h>
-#include <stdlib.h>
 
 namespace moe {
 namespace gemm8 {
@@ -156,8 +155,11 @@ __device__ __forceinline__ bool mbar_wait_inline(uint32_t bar, uint32_t parity, 
 struct Tile {
   int e, row0, row_end, n_tile;
 };
-// tstart[e] = row tiles of the groups before e.  Tile ids: group, then column tile, then row tile, so that CTAs side by side
-// read one B tile.
+// tstart[e] = row tiles of the groups before e.  Tile ids: group, then bands of eight column tiles, then row tile, then column
+// tile, so that what the SMs work on at a time is a block of the output that is neither tall nor wide, and its rows of A and
+// B stay in L2 meanwhile (column tiles one after the other -> this: 8192 x 4096 x 7168 247 -> 235 us, 32768 rows on 64 experts of
+// 2048 x 7168, Zipf load, 669 -> 573 us; four or sixteen tiles to a band are no better).
+constexpr int BAND = 8;
 __device__ __forceinline__ Tile decode_tile(int id, const int32_t* tstart, const int32_t* offs, int E, int NT) {
   int lo = 0, hi = E - 1;
   while (lo < hi) {
@@ -165,10 +167,11 @@ __device__ __forceinline__ Tile decode_tile(int id, const int32_t* tstart, const
     if (tstart[mid + 1] * NT > id) hi = mid; else lo = mid + 1;
   }
   const int local = id - tstart[lo] * NT, mt = tstart[lo + 1] - tstart[lo];
+  const int band = local / (mt * BAND), in = local - band * mt * BAND, width = min(BAND, NT - band * BAND), m = in / width;
   Tile t;
   t.e = lo;
-  t.n_tile = local / mt;
-  t.row0 = offs[lo] + (local - t.n_tile * mt) * BM;
+  t.n_tile = band * BAND + in - m * width;
+  t.row0 = offs[lo] + m * BM;
   t.row_end = offs[lo + 1];
   return t;
 }
@@ -242,7 +245,7 @@ __device__ __forceinline__ void store_rows(const Params& p, int row0, int row_en
     return;
   }
   // rows of no alignment: 16 columns at a time through shared memory, from where half a warp writes neighbours of one row
-  // (188 x 7699 x 464: 25.1 -> %ODD% us)
+  // (188 x 7699 x 464: 25.1 -> 9.6 us)
   const int n_rows = min(32, row_end - row0), cc = lane & 15;
 #pragma unroll
   for (int c = 0; c < COLS / 16; ++c) {
@@ -428,13 +431,16 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       f32x2 acc[COLS / 2];
 #pragma unroll
       for (int j = 0; j < COLS / 2; ++j) acc[j] = 0ull;
-      float s_next = *sa * *sb;
+      // the scales of the next block are on their way while this one is added: their product waits for its turn, because taking
+      // it at once would hold the warp for the latency of the loads in every block
+      float a_next = *sa, b_next = *sb;
       for (int kb = kb0; kb < kb1; ++kb) {
-        const float s = s_next;
+        const float s = a_next * b_next;
         if (kb + 1 < kb1) {
           sa += p.sa_k;
           ++sb;
-          s_next = *sa * *sb;
+          a_next = *sa;
+          b_next = *sb;
         }
         if (!mbar_wait_inline(tfull0 + 8 * buf, buf_phase, abort_flag, p.status, 34)) { ok = false; break; }
         tc_fence_after();
@@ -580,15 +586,16 @@ extern "C" int moe_fp8_gemm(const void* A, int64_t lda, const float* a_scale, in
   p.vec_store = !(reinterpret_cast<uintptr_t>(Y) & 15) && (ldy * el) % 16 == 0 && (N * el) % 16 == 0;
   if (p.vec_store && !(reinterpret_cast<uintptr_t>(Y) & 31) && (ldy * el) % 32 == 0 && (N * el) % 32 == 0) p.vec_store = 2;
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  // Tiles of 256 or of 128 columns: a k-block of the wider takes about 9 / 5 the time of one of the narrower, and the launch as
-  // many rounds of tiles as the SMs need.  Where even the narrow tiles leave SMs idle, clusters of 2, 4 or 8 CTAs share the
-  // k-blocks of a tile (clusters of 4 and 8 do not fill the GPU: counted as 128 SMs), two k-blocks each at least.
+  // Tiles of 256 or of 128 columns: a round of the wider takes about 3 / 2 the time of one of the narrower (us, wide / narrow:
+  // 512 x 4096 x 4096, one round each, 21.4 / 16.0; 2500 x 2048 x 2048, two and three, 23.5 / 23.4; 1024 x 4096 x 4096, one and two, 21.8 /
+  // 27.1), and the launch as many rounds of tiles as the SMs need.  Where even the narrow tiles leave SMs idle, clusters of 2, 4
+  // or 8 CTAs share the k-blocks of a tile (clusters of 4 and 8 do not fill the GPU: counted as 128 SMs), two k-blocks each at
+  // least.  A token through 4096 x 7168: 35 us on 16 wide tiles, 11.8 on 32 clusters of 4.
   const int64_t m_tiles = offsets ? rows / BM + (rows < E ? rows : E) : ceil_div64(rows, BM);
   const int64_t tiles256 = m_tiles * ceil_div64(N, 256), tiles128 = m_tiles * ceil_div64(N, 128);
   if (tiles128 > 0x7FFFFFFFll) return fail(MOE_ERR_UNSUPPORTED, "fp8_gemm: too many tiles");
   p.a_box_rows = rows < BM ? (int)(rows + 7) / 8 * 8 : BM;
-  static const int forced = [] { const char* f = getenv("F8BN"); return f ? atoi(f) : 0; }();
-  if (forced != 128 && (forced == 256 || ceil_div64(tiles256, dev.sm_count) * 5 <= ceil_div64(tiles128, dev.sm_count) * 4))
+  if (ceil_div64(tiles256, dev.sm_count) * 3 <= ceil_div64(tiles128, dev.sm_count) * 2)
     return launch<256, false>(A, lda, B, p, tiles256, 1, dev.sm_count, st);
   int split = 1;
   while (split < MAX_SPLIT && p.k_blocks >= 4 * split && tiles128 * split * 2 <= (split == 1 ? dev.sm_count : dev.sm_count * 7 / 8)) split *= 2;

@@ -18,6 +18,7 @@ from . import _lib, ops
 
 GROUP = 128
 E4M3 = torch.float8_e4m3fn
+_OUT_DTYPES = (None, torch.bfloat16, torch.float16, torch.float32)
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # MOE_DTYPE_* of include/moe_b200.h
 
 
@@ -94,48 +95,54 @@ def fp8_quantize_blocks(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     return q, scale
 
 
-def _product(a, a_scale, b, b_scale, offsets, out_dtype, out) -> torch.Tensor:
+def _product(a, a_scale, b, b_scale, E, offsets, out_dtype, out) -> torch.Tensor:
+    """b [N, K] and b_scale without their leading E where offsets is None."""
     ops._need_cuda(a, a_scale, b, b_scale, offsets, out)
     if a.dtype != E4M3 or b.dtype != E4M3:
         raise ValueError("a and b must be float8_e4m3fn")
-    if a.dim() != 2 or b.dim() != 3:
-        raise ValueError("a must be [M, K], b [N, K] (fp8_gemm) or [E, N, K] (fp8_grouped_gemm)")
-    (M, K), (E, N, K2) = a.shape, b.shape
+    if a.dim() != 2:
+        raise ValueError("a must be [M, K]")
+    M, K = a.shape
+    N, K2 = b.shape[-2:]
     if K2 != K:
         raise ValueError(f"inner dimensions differ: a has K={K}, b has K={K2}")
     if K < 16 or K % 16 or N < 1 or E < 1:
         raise ValueError(f"K={K} must be a positive multiple of 16, N={N} and E={E} positive")
-    if a_scale.dtype != torch.float32 or tuple(a_scale.shape) != (M, _groups(K)):
-        raise ValueError(f"a_scale must be float32 [{M}, {_groups(K)}]")
-    if b_scale.dtype != torch.float32 or tuple(b_scale.shape) != (E, _groups(N), _groups(K)):
-        raise ValueError(f"b_scale must be float32 {'' if offsets is None else f'{E} x '}[{_groups(N)}, {_groups(K)}]")
+    kb, nb = _groups(K), _groups(N)
+    if a_scale.dtype != torch.float32 or a_scale.shape != (M, kb):
+        raise ValueError(f"a_scale must be float32 [{M}, {kb}]")
+    if b_scale.dtype != torch.float32 or b_scale.shape != ((nb, kb) if offsets is None else (E, nb, kb)):
+        raise ValueError(f"b_scale must be float32 [{'' if offsets is None else f'{E}, '}{nb}, {kb}]")
     dev = a.device
     for t in (a_scale, b, b_scale, offsets, out):
         if t is not None and t.device != dev:
             raise ValueError(f"all tensors must be on one device, not on {dev} and {t.device}")
-    if offsets is not None and (offsets.dtype != torch.int32 or tuple(offsets.shape) != (E + 1,)):
-        raise ValueError(f"offsets must be int32 [{E + 1}]")
-    if out is not None:
-        if tuple(out.shape) != (M, N) or out.dtype not in _DTYPES or (M > 0 and N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
-            raise ValueError(f"out must be [{M}, {N}] in bfloat16, float16 or float32 with packed rows that do not overlap")
-        if out_dtype is not None and out_dtype != out.dtype:
-            raise ValueError(f"out is {out.dtype}, not {out_dtype}")
-    elif out_dtype not in (None, *_DTYPES):
-        raise ValueError("out_dtype must be bfloat16, float16 or float32")
-    if a.stride(1) != 1 or a.data_ptr() & 15 or _stride(a) < K or _stride(a) % 16:
-        a = a.clone(memory_format=torch.contiguous_format)
-    if not b.is_contiguous() or b.data_ptr() & 15:
-        b = b.clone(memory_format=torch.contiguous_format)
-    b_scale = b_scale.contiguous()
     if offsets is not None:
+        if offsets.dtype != torch.int32 or offsets.shape != (E + 1,):
+            raise ValueError(f"offsets must be int32 [{E + 1}]")
         offsets = offsets.contiguous()
     fresh = out is None
     if fresh:
-        out = torch.empty(M, N, dtype=out_dtype or torch.bfloat16, device=dev)
+        if out_dtype not in _OUT_DTYPES:
+            raise ValueError("out_dtype must be bfloat16, float16 or float32")
+        out = a.new_empty((M, N), dtype=out_dtype or torch.bfloat16)
+    else:
+        if out.shape != (M, N) or out.dtype not in _DTYPES or (M > 0 and N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
+            raise ValueError(f"out must be [{M}, {N}] in bfloat16, float16 or float32 with packed rows that do not overlap")
+        if out_dtype is not None and out_dtype != out.dtype:
+            raise ValueError(f"out is {out.dtype}, not {out_dtype}")
+    lda = _stride(a)
+    if a.stride(1) != 1 or a.data_ptr() & 15 or lda < K or lda % 16:
+        a = a.clone(memory_format=torch.contiguous_format)
+        lda = K
+    if not b.is_contiguous() or b.data_ptr() & 15:
+        b = b.clone(memory_format=torch.contiguous_format)
+    b_scale = b_scale.contiguous()
+    lib = _lib.load()
     with ops._on(dev):
-        rc = _lib.load().moe_fp8_gemm(ops._ptr(a), _stride(a), ops._ptr(a_scale), a_scale.stride(0), a_scale.stride(1), ops._ptr(b),
-                                      ops._ptr(b_scale), ops._ptr(offsets), M, K, N, E, ops._ptr(out), _stride(out), _DTYPES[out.dtype],
-                                      int(fresh), ops._ptr(ops.status_buffer(dev)), ops._stream())
+        rc = lib.moe_fp8_gemm(a.data_ptr(), lda, a_scale.data_ptr(), *a_scale.stride(), b.data_ptr(), b_scale.data_ptr(),
+                              ops._ptr(offsets), M, K, N, E, out.data_ptr(), N if fresh else _stride(out), _DTYPES[out.dtype], int(fresh),
+                              ops.status_buffer(dev).data_ptr(), ops._stream())
     _lib.check(rc, "moe_fp8_gemm")
     ops._after(dev)
     return out
@@ -146,9 +153,9 @@ def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
     """y [M, N] = (a * a_scale) @ (b * b_scale).T: a e4m3 [M, K] with a_scale float32 [M, ceil(K / 128)] (fp8_quantize), b e4m3
     [N, K] with b_scale float32 [ceil(N / 128), ceil(K / 128)] (fp8_quantize_blocks); K a multiple of 16.  Accumulated in
     fp32, rounded once to out_dtype: bfloat16 (the default), float16 or float32."""
-    if b.dim() != 2 or b_scale.dim() != 2:
-        raise ValueError("b must be [N, K] and b_scale [ceil(N / 128), ceil(K / 128)]")
-    return _product(a, a_scale, b.unsqueeze(0), b_scale.unsqueeze(0), None, out_dtype, out)
+    if b.dim() != 2:
+        raise ValueError("b must be [N, K]")
+    return _product(a, a_scale, b, b_scale, 1, None, out_dtype, out)
 
 
 def fp8_grouped_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, offsets: torch.Tensor,
@@ -156,6 +163,6 @@ def fp8_grouped_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_
     """y[r] = fp8_gemm with b[e] for the rows offsets[e] .. offsets[e + 1] - 1 of every expert e: b e4m3 [E, N, K] with b_scale
     float32 [E, ceil(N / 128), ceil(K / 128)], offsets int32 [E + 1] on the device (no host synchronisation).  Rows of no
     expert (behind offsets[E]) are zero in a new tensor and left as they were in ``out``."""
-    if offsets is None:
-        raise ValueError("offsets must be int32 [E + 1]")
-    return _product(a, a_scale, b, b_scale, offsets, out_dtype, out)
+    if offsets is None or b.dim() != 3:
+        raise ValueError("b must be [E, N, K] and offsets int32 [E + 1]")
+    return _product(a, a_scale, b, b_scale, b.shape[0], offsets, out_dtype, out)
