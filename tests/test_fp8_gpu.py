@@ -369,3 +369,78 @@ def test_expert_layer_in_graphs_and_on_streams(cuda, lib):
     side.synchronize()
     assert torch.equal(got, layers[0][2]) and torch.equal(want, layers[1][2])
     ops.check_status(cuda)
+
+
+# ------------------------------------------------------------------------------------------------------- more shapes
+@pytest.mark.parametrize("out_dtype", DTYPES)
+@pytest.mark.parametrize("M,N,K", [(5000, 1000, 272), (4100, 1001, 128), (2000, 4500, 256), (128, 2304, 1536), (33, 640, 3600), (32, 640, 2048),
+                                   (31, 129, 1296), (97, 1024, 512), (1, 8192, 1024), (640, 2176, 160), (20000, 136, 16)])
+def test_gemm_of_every_tiling_is_exact(cuda, lib, M, N, K, out_dtype):
+    """Wide tiles in several rounds and bands, narrow ones, clusters of 2, 4 and 8, few rows, and widths without vectors."""
+    g = torch.Generator(device=cuda).manual_seed(M + N)
+    a, sa, b, sb = _whole(M, N, K, 1, g, cuda)
+    y = kernels.fp8_gemm(a, sa, b[0], sb[0], out_dtype=out_dtype)
+    ops.check_status(cuda)
+    assert torch.equal(y, _product(a, sa, b[0], sb[0])[0].float().to(out_dtype))
+    # into rows of a wider tensor: other alignments, nothing beside them changes
+    for left in (0, 1, 4):
+        room = torch.full((M, N + 8), 7.0, dtype=out_dtype, device=cuda)
+        kernels.fp8_gemm(a, sa, b[0], sb[0], out=room[:, left:left + N])
+        assert torch.equal(room[:, left:left + N], y)
+        room[:, left:left + N] = 7
+        assert torch.all(room == 7)
+
+
+@pytest.mark.parametrize("M,N,K,E", [(3000, 1500, 400, 20), (9000, 2056, 144, 37), (32, 512, 1024, 12), (20, 2048, 768, 256), (2048, 1024, 256, 1024)])
+def test_grouped_gemm_of_every_tiling_is_exact(cuda, lib, M, N, K, E):
+    g = torch.Generator(device=cuda).manual_seed(M + N + E)
+    a, sa, b, sb = _whole(M, N, K, E, g, cuda)
+    sizes = _group_sizes("ragged", M, E, torch.Generator().manual_seed(M))
+    at = torch.tensor([0] + sizes).cumsum(0)
+    y = kernels.fp8_grouped_gemm(a, sa, b, sb, at.int().to(cuda))
+    ops.check_status(cuda)
+    want = torch.zeros(M, N, dtype=torch.float64, device=cuda)
+    for e in range(E):
+        if sizes[e]:
+            part = slice(int(at[e]), int(at[e + 1]))
+            want[part] = _product(a[part], sa[part], b[e], sb[e])[0]
+    assert torch.equal(y, want.float().bfloat16())
+
+
+def test_first_group_may_start_behind_the_first_row(cuda, lib):
+    g = torch.Generator(device=cuda).manual_seed(8)
+    a, sa, b, sb = _whole(300, 256, 256, 2, g, cuda)
+    y = kernels.fp8_grouped_gemm(a, sa, b, sb, torch.tensor([40, 200, 260], dtype=torch.int32, device=cuda))
+    assert torch.all(y[:40] == 0) and torch.all(y[260:] == 0)
+    assert torch.equal(y[40:200], _product(a[40:200], sa[40:200], b[0], sb[0])[0].float().bfloat16())
+    assert torch.equal(y[200:260], _product(a[200:260], sa[200:260], b[1], sb[1])[0].float().bfloat16())
+
+
+def test_products_on_two_streams_at_once(cuda, lib):
+    """Nothing is shared between calls: products that overlap on the device give what they give alone."""
+    g = torch.Generator(device=cuda).manual_seed(9)
+    jobs = []
+    for M, N, K in ((1500, 2048, 2048), (16, 4096, 4096)):
+        a, sa, b, sb = _whole(M, N, K, 1, g, cuda)
+        jobs.append((a, sa, b[0], sb[0], kernels.fp8_gemm(a, sa, b[0], sb[0])))
+    torch.cuda.synchronize(cuda)
+    streams = [torch.cuda.Stream(cuda) for _ in jobs]
+    got = [[], []]
+    for _ in range(20):
+        for (a, sa, b, sb, _), stream, out in zip(jobs, streams, got):
+            with torch.cuda.stream(stream):
+                out.append(kernels.fp8_gemm(a, sa, b, sb))
+    torch.cuda.synchronize(cuda)
+    for job, out in zip(jobs, got):
+        assert all(torch.equal(y, job[4]) for y in out)
+    ops.check_status(cuda)
+
+
+def test_results_repeat_bit_by_bit(cuda, lib):
+    g = torch.Generator(device=cuda).manual_seed(10)
+    for M, N, K in ((3, 512, 7168), (700, 2048, 4096)):
+        a, sa = kernels.fp8_quantize(torch.randn(M, K, generator=g, device=cuda))
+        b, sb = kernels.fp8_quantize_blocks(torch.randn(N, K, generator=g, device=cuda))
+        y = kernels.fp8_gemm(a, sa, b, sb, out_dtype=torch.float32)
+        for _ in range(5):
+            assert torch.equal(kernels.fp8_gemm(a, sa, b, sb, out_dtype=torch.float32), y)

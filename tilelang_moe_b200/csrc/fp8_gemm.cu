@@ -6,11 +6,17 @@
 // memory), and because the scales change every 128 k, each block's sum leaves tensor memory and is added, scaled, to fp32
 // accumulators in registers:
 //
-//   warp 0      TMA producer: per k-block one A box (128 rows x 128 bytes) and one B box (BN rows), 128-byte swizzle, into a
-//               ring of shared-memory stages;
+//   warp 0      TMA producer: per k-block one A box (128 rows x 128 bytes, 32 for a tile of few rows) and one B box (BN rows),
+//               128-byte swizzle, into a ring of shared-memory stages;
 //   warp 1      MMA issuer: four instructions (K = 32) per k-block into one of two accumulators in tensor memory, in turn;
 //   warps 2..9  one tile row and half of the tile's columns per thread: acc += (sa * sb) * block sum, while the other
 //               accumulator is being filled; after the last block convert and store.
+//
+// What bounds it.  Many rows: the power cap.  8192 x 4096 x 7168 takes 235 to 275 us (2.05 to 1.75 PFLOP/s) with the clocks at 1.45 to
+// 1.5 GHz and 1000 W; the same kernel without its additions, on a pair of CTAs, 170, and the library's product without block
+// scales 167 to 200.  An accumulating warp needs about 500 of the 870 clocks of a k-block.  A form on CTA pairs (cta_group::2, half the B
+// traffic per SM) was no faster with the additions: 238 against 247 us here, 146 against 137 at 8192 x 7168 x 2048, 602 against 583 on 64 experts.
+// Few rows: reading the weights: 256 rows on 128 experts of 2048 x 4096 in 156 us, 6.1 TB/s.
 //
 // K need not be a multiple of 128: TMA fills what lies behind it with zeros.  Rows of a tile behind its group are computed
 // and not stored.  Every barrier wait is bounded in time, as in the 16-bit kernels.
@@ -179,12 +185,26 @@ __device__ __forceinline__ Tile decode_tile(int id, const int32_t* tstart, const
   t.row_end = offs[lo + 1];
   return t;
 }
-__device__ __forceinline__ int group_tiles(const int32_t* offs, int e) {
-  return max(0, offs[e + 1] - offs[e] + BM - 1) / BM;
-}
-__device__ __forceinline__ void tile_prefix(int32_t* tstart, const int32_t* offs, int E, int lane) {
-  const int per = (E + 31) / 32;
-  const int e_lo = min(E, lane * per), e_hi = min(E, e_lo + per);
+__device__ __forceinline__ int group_tiles(const int32_t* offs, int e) { return (offs[e + 1] - offs[e] + BM - 1) / BM; }
+
+// One warp: offs[0 .. E] made a prefix sum of groups inside the tensor (every entry cut to [0, rows] already, none below the one
+// before it), so that a table that is none leaves every access in bounds; then the row tiles before each group.
+__device__ __forceinline__ void tile_prefix(int32_t* tstart, int32_t* offs, int E, int lane) {
+  const int per = (E + 32) / 32;
+  const int lo = min(E + 1, lane * per), hi = min(E + 1, lo + per);
+  int top = 0;
+  for (int i = lo; i < hi; ++i) offs[i] = top = max(top, offs[i]);
+  int before = top;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xFFFFFFFFu, before, o);
+    if (lane >= o) before = max(before, v);
+  }
+  before = __shfl_up_sync(0xFFFFFFFFu, before, 1);
+  if (lane > 0)
+    for (int i = lo; i < hi; ++i) offs[i] = max(before, offs[i]);
+  __syncwarp();
+  const int e_lo = min(E, lo), e_hi = min(E, hi);
   int sum = 0;
   for (int e = e_lo; e < e_hi; ++e) sum += group_tiles(offs, e);
   int inc = sum;
@@ -352,7 +372,6 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     tmem_alloc(smem_u32(tmem_slot), C::TMEM_COLS);
     tmem_relinquish();
   }
-  // a table that is no prefix sum leaves every access inside the tensors: starts and ends are cut to [0, rows]
   for (int e = threadIdx.x; e <= E; e += blockDim.x) offs[e] = p.offsets ? min(max(p.offsets[e], 0), p.rows) : (e == 0 ? 0 : p.rows);
   __syncthreads();
   if (warp == 2) tile_prefix(tstart, offs, E, lane);
