@@ -52,12 +52,12 @@ def fp8_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     K = x.shape[-1]
     q = x.new_empty(x.shape, dtype=E4M3)
     scale = x.new_empty((*x.shape[:-1], _groups(K)), dtype=torch.float32)
-    rows = _rows2(x)
-    with ops._on(x.device):
-        rc = _lib.load().moe_fp8_quantize_rows(ops._ptr(rows), _stride(rows), rows.shape[0], K, dt, ops._ptr(q), ops._ptr(scale),
+    rows, dev = _rows2(x), x.device
+    with ops._on(dev):
+        rc = _lib.load().moe_fp8_quantize_rows(rows.data_ptr(), _stride(rows), rows.shape[0], K, dt, q.data_ptr(), scale.data_ptr(),
                                                ops._stream())
     _lib.check(rc, "moe_fp8_quantize_rows")
-    ops._after(x.device)
+    ops._after(dev)
     return q, scale
 
 
@@ -71,12 +71,12 @@ def fp8_silu_mul(gate: torch.Tensor, up: torch.Tensor) -> Tuple[torch.Tensor, to
     I = gate.shape[-1]
     q = gate.new_empty(gate.shape, dtype=E4M3)
     scale = gate.new_empty((*gate.shape[:-1], _groups(I)), dtype=torch.float32)
-    g, u = _rows2(gate), _rows2(up)
-    with ops._on(gate.device):
-        rc = _lib.load().moe_fp8_silu_mul(ops._ptr(g), _stride(g), ops._ptr(u), _stride(u), g.shape[0], I, dt, ops._ptr(q), ops._ptr(scale),
-                                          ops._stream())
+    g, u, dev = _rows2(gate), _rows2(up), gate.device
+    with ops._on(dev):
+        rc = _lib.load().moe_fp8_silu_mul(g.data_ptr(), _stride(g), u.data_ptr(), _stride(u), g.shape[0], I, dt, q.data_ptr(),
+                                          scale.data_ptr(), ops._stream())
     _lib.check(rc, "moe_fp8_silu_mul")
-    ops._after(gate.device)
+    ops._after(dev)
     return q, scale
 
 

@@ -29,12 +29,14 @@ class MoESort:
     k: int                   # entries per token
 
     def __post_init__(self):
-        for name, t, least in (("offsets", self.offsets, 2), ("perm", self.perm, 0), ("row_of", self.row_of, 0)):
-            if t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous() or t.numel() < least:
-                raise ValueError(f"{name} must be a contiguous int32 vector")
-        if self.k < 1 or self.row_of.numel() % self.k or self.perm.numel() != self.row_of.numel():
+        offsets, perm, row_of = self.offsets, self.perm, self.row_of
+        if not (offsets.dtype is perm.dtype is row_of.dtype is torch.int32 and offsets.dim() == perm.dim() == row_of.dim() == 1
+                and offsets.is_contiguous() and perm.is_contiguous() and row_of.is_contiguous() and offsets.numel() > 1):
+            raise ValueError("offsets, perm and row_of must be contiguous int32 vectors, offsets of two entries at least")
+        n = row_of.numel()
+        if self.k < 1 or n % self.k or perm.numel() != n:
             raise ValueError(f"perm and row_of must have {self.k} entries for each token")
-        if not (self.offsets.device == self.perm.device == self.row_of.device):
+        if not (offsets.device == perm.device == row_of.device):
             raise ValueError("the tables of a sort must be on one device")
 
     @classmethod
@@ -87,28 +89,35 @@ def _stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _live(sort: MoESort) -> int:
+    """Address of offsets[E]: the rows that hold an entry."""
+    return sort.offsets.data_ptr() + 4 * (sort.offsets.numel() - 1)
+
+
 def _permute(x: torch.Tensor, sort: MoESort) -> torch.Tensor:
     x = _rows(x)
     T, H = x.shape
-    w = x.element_size()
-    out = x.new_empty((T * sort.k, H))
-    with ops._on(x.device):
-        rc = _lib.load().moe_permute(ops._ptr(x), _stride(x) * w, H * w, ops._ptr(sort.row_of), ops._ptr(sort.offsets) + 4 * sort.n_experts,
-                                     T, sort.k, ops._ptr(out), ops._stream())
+    k, w, dev = sort.k, x.element_size(), x.device
+    out = x.new_empty((T * k, H))
+    with ops._on(dev):
+        rc = _lib.load().moe_permute(x.data_ptr(), _stride(x) * w, H * w, sort.row_of.data_ptr(), _live(sort), T, k, out.data_ptr(),
+                                     ops._stream())
     _lib.check(rc, "moe_permute")
-    ops._after(x.device)
+    ops._after(dev)
     return out
 
 
 def _unpermute(rows: torch.Tensor, sort: MoESort, weights: Optional[torch.Tensor]) -> torch.Tensor:
     rows = _rows(rows)
-    T, H = sort.tokens, rows.shape[1]
+    n, H = rows.shape
+    k, dev = sort.k, rows.device
+    T = n // k
     out = rows.new_empty((T, H))
-    with ops._on(rows.device):
-        rc = _lib.load().moe_unpermute(ops._ptr(rows), _stride(rows), ops._ptr(sort.row_of), ops._ptr(sort.offsets) + 4 * sort.n_experts,
-                                       ops._ptr(weights), T, sort.k, H, _DTYPES[rows.dtype], ops._ptr(out), ops._stream())
+    with ops._on(dev):
+        rc = _lib.load().moe_unpermute(rows.data_ptr(), _stride(rows), sort.row_of.data_ptr(), _live(sort), ops._ptr(weights), T, k, H,
+                                       _DTYPES[rows.dtype], out.data_ptr(), ops._stream())
     _lib.check(rc, "moe_unpermute")
-    ops._after(rows.device)
+    ops._after(dev)
     return out
 
 
@@ -116,14 +125,15 @@ def _unpermute_grad(gy: torch.Tensor, rows: Optional[torch.Tensor], sort: MoESor
                     want_weights: bool):
     gy = _rows(gy)
     T, H = gy.shape
-    g_rows = torch.empty(T * sort.k, H, dtype=gy.dtype, device=gy.device) if want_rows else None
-    g_w = torch.empty(T, sort.k, dtype=torch.float32, device=gy.device) if want_weights else None
-    with ops._on(gy.device):
-        rc = _lib.load().moe_unpermute_grad(ops._ptr(gy), _stride(gy), ops._ptr(rows), 0 if rows is None else _stride(rows),
-                                            ops._ptr(sort.row_of), ops._ptr(sort.offsets) + 4 * sort.n_experts, ops._ptr(weights), T,
-                                            sort.k, H, _DTYPES[gy.dtype], ops._ptr(g_rows), ops._ptr(g_w), ops._stream())
+    k, dev = sort.k, gy.device
+    g_rows = gy.new_empty((T * k, H)) if want_rows else None
+    g_w = weights.new_empty((T, k)) if want_weights else None
+    with ops._on(dev):
+        rc = _lib.load().moe_unpermute_grad(gy.data_ptr(), _stride(gy), ops._ptr(rows), 0 if rows is None else _stride(rows),
+                                            sort.row_of.data_ptr(), _live(sort), weights.data_ptr(), T, k, H, _DTYPES[gy.dtype],
+                                            ops._ptr(g_rows), ops._ptr(g_w), ops._stream())
     _lib.check(rc, "moe_unpermute_grad")
-    ops._after(gy.device)
+    ops._after(dev)
     return g_rows, g_w
 
 
@@ -157,18 +167,14 @@ class _Unpermute(torch.autograd.Function):
         return (*_unpermute_grad(gy, rows, ctx.sort, weights, ctx.needs_input_grad[0], ctx.needs_input_grad[1]), None)
 
 
-def _same_device(sort: MoESort, t: torch.Tensor, what: str) -> None:
-    if t.device != sort.row_of.device:
-        raise ValueError(f"{what} is on {t.device}, the sort's tables on {sort.row_of.device}")
-
-
 def moe_permute(x: torch.Tensor, sort: MoESort) -> torch.Tensor:
     """Rows of x [T, H] at their entries' places: [T*k, H] of x's type.  Any element type; floating types of 16 and 32 bits
     have a gradient, others (8-bit values beside their scales, say) are copied."""
     ops._need_cuda(x)
-    if x.dim() != 2 or x.shape[1] < 1 or x.shape[0] != sort.tokens:
+    if x.dim() != 2 or x.shape[1] < 1 or x.shape[0] * sort.k != sort.row_of.numel():
         raise ValueError(f"x must be [{sort.tokens}, H], one row for each token of the sort")
-    _same_device(sort, x, "x")
+    if x.device != sort.row_of.device:
+        raise ValueError(f"x is on {x.device}, the sort's tables on {sort.row_of.device}")
     if x.requires_grad and torch.is_grad_enabled():
         if x.dtype not in _DTYPES:
             raise ValueError("the gradient of moe_permute is computed in bfloat16, float16 or float32")
@@ -182,13 +188,14 @@ def moe_unpermute(rows: torch.Tensor, sort: MoESort, weights: Optional[torch.Ten
     ops._need_cuda(rows, weights)
     if rows.dtype not in _DTYPES:
         raise ValueError("rows must be bfloat16, float16 or float32")
-    if rows.dim() != 2 or rows.shape[1] < 1 or rows.shape[0] != sort.tokens * sort.k:
-        raise ValueError(f"rows must be [{sort.tokens * sort.k}, H], one for each entry of the sort")
-    _same_device(sort, rows, "rows")
+    n, k, dev = sort.row_of.numel(), sort.k, sort.row_of.device
+    if rows.dim() != 2 or rows.shape[1] < 1 or rows.shape[0] != n:
+        raise ValueError(f"rows must be [{n}, H], one for each entry of the sort")
+    if rows.device != dev or (weights is not None and weights.device != dev):
+        raise ValueError(f"rows and weights must be on the device of the sort's tables, {dev}")
     if weights is not None:
-        if weights.dtype != torch.float32 or tuple(weights.shape) != (sort.tokens, sort.k):
-            raise ValueError(f"routing weights must be float32 [{sort.tokens}, {sort.k}]")
-        _same_device(sort, weights, "weights")
+        if weights.dtype != torch.float32 or weights.shape != (n // k, k):
+            raise ValueError(f"routing weights must be float32 [{n // k}, {k}]")
         weights = weights.contiguous()
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
         return _Unpermute.apply(rows, weights, sort)
