@@ -453,10 +453,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
     for (int tile = first_tile; ok && tile < total_tiles; tile += tile_step) {
       // this thread's scales, and as little else as possible: the accumulators leave hardly any register for the loop
       const float *sa = p.sa + kb0 * p.sa_k, *sb;
+      bool any_row;                                   // rows of the warp that are the group's: without one there is nothing to add
       {
         const Tile t = decode_tile(tile, tstart, offs, E, NT);
         const int row = t.row0 + q * 32 + lane;
         if (row < t.row_end) sa += (int64_t)row * p.sa_row;
+        any_row = t.row0 + q * 32 < t.row_end;
         // columns behind N have no scale block of their own: the last one stands in, nothing of them is stored
         sb = p.sb + ((int64_t)t.e * p.n_blocks + min((t.n_tile * BN + half * COLS) / 128, p.n_blocks - 1)) * p.k_blocks + kb0;
       }
@@ -478,12 +480,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         tc_fence_after();
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + half * COLS);
         const f32x2 s2 = pair_of(s, s);
+        if (any_row) {
 #pragma unroll
-        for (int c = 0; c < COLS / 16; ++c) {
-          f32x2 v[8];
-          tmem_ld16_pairs(taddr + c * 16, v);
+          for (int c = 0; c < COLS / 16; ++c) {
+            f32x2 v[8];
+            tmem_ld16_pairs(taddr + c * 16, v);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) fma2(acc[c * 8 + j], v[j], s2);
+            for (int j = 0; j < 8; ++j) fma2(acc[c * 8 + j], v[j], s2);
+          }
         }
         tc_fence_before();
         __syncwarp();
