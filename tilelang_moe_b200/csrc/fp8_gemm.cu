@@ -12,11 +12,12 @@
 //   warps 2..9  one tile row and half of the tile's columns per thread: acc += (sa * sb) * block sum, while the other
 //               accumulator is being filled; after the last block convert and store.
 //
-// What bounds it.  Many rows: the power cap.  8192 x 4096 x 7168 takes 235 to 275 us (2.05 to 1.75 PFLOP/s) with the clocks at 1.45 to
-// 1.5 GHz and 1000 W; the same kernel without its additions, on a pair of CTAs, 170, and the library's product without block
-// scales 167 to 200.  An accumulating warp needs about 500 of the 870 clocks of a k-block.  A form on CTA pairs (cta_group::2, half the B
-// traffic per SM) was no faster with the additions: 238 against 247 us here, 146 against 137 at 8192 x 7168 x 2048, 602 against 583 on 64 experts.
-// Few rows: reading the weights: 256 rows on 128 experts of 2048 x 4096 in 156 us, 6.1 TB/s.
+// What bounds it.  Many rows: the power cap.  8192 x 4096 x 7168 takes 231 us from idle and 269 back to back (2.08 and 1.79 PFLOP/s)
+// with the clocks at 1.45 to 1.5 GHz and 1000 W; the library's product without block scales 167 and 200.  An accumulating warp
+// needs about 500 of the 870 clocks of a k-block.  A form on CTA pairs (cta_group::2, two thirds of the operand traffic per SM) ran
+// at the tensor cores' 512 clocks a k-block without the additions, but with them was no faster: 265 to 288 us against 269 here, 160 to
+// 172 against 162 at 8192 x 7168 x 2048, 667 to 725 against 650 on 64 experts.  Sixteen accumulating warps instead of eight: 307 against 258.
+// Few rows: reading the weights: 250 rows on 111 experts of 2048 x 4096 in 166 us, 5.6 TB/s.
 //
 // K need not be a multiple of 128: TMA fills what lies behind it with zeros.  Rows of a tile behind its group are computed
 // and not stored.  Every barrier wait is bounded in time, as in the 16-bit kernels.
