@@ -236,6 +236,7 @@ def test_gemm_of_nothing_and_of_what_is_no_number(cuda, lib):
     a, sa, b, sb = _whole(130, 140, 256, 2, g, cuda)
     assert kernels.fp8_gemm(a[:0], sa[:0], b[0], sb[0]).shape == (0, 140)
     none = torch.zeros(3, dtype=torch.int32, device=cuda)
+    assert kernels.fp8_grouped_gemm(a[:0], sa[:0], b, sb, none).shape == (0, 140)
     assert torch.all(kernels.fp8_grouped_gemm(a, sa, b, sb, none) == 0)
     # a NaN in one row of a, in one row of b, in a scale: they reach their row, column and rows, nothing else
     want = kernels.fp8_gemm(a, sa, b[0], sb[0])
@@ -444,3 +445,47 @@ def test_results_repeat_bit_by_bit(cuda, lib):
         y = kernels.fp8_gemm(a, sa, b, sb, out_dtype=torch.float32)
         for _ in range(5):
             assert torch.equal(kernels.fp8_gemm(a, sa, b, sb, out_dtype=torch.float32), y)
+
+
+def test_bytes_around_the_operands_do_not_matter(cuda, lib):
+    """a and b are views whose surroundings are NaN in every byte: what lies behind K, behind the last row and in the next
+    expert's place is not multiplied."""
+    g = torch.Generator(device=cuda).manual_seed(11)
+    M, N, K = 77, 130, 208
+    a, sa, b, sb = _whole(M, N, K, 1, g, cuda)
+    wide = torch.full((M + 60, K + 48), 0x7F, dtype=torch.uint8, device=cuda)
+    wide[30:30 + M, 16:16 + K] = a.view(torch.uint8)
+    more = torch.full((3, N, K), 0x7F, dtype=torch.uint8, device=cuda)
+    more[1] = b[0].view(torch.uint8)
+    scales = torch.full((3, 2, 2), float("nan"), device=cuda)
+    scales[1] = sb[0]
+    around = torch.full((M + 2, 4), float("nan"), device=cuda)
+    around[1:M + 1, 1:3] = sa
+    want = _product(a, sa, b[0], sb[0])[0].float().bfloat16()
+    view = wide[30:30 + M, 16:16 + K].view(E4M3)
+    assert torch.equal(kernels.fp8_gemm(view, around[1:M + 1, 1:3], more[1].view(E4M3), scales[1]), want)
+    offsets = torch.tensor([0, 0, M, M], dtype=torch.int32, device=cuda)
+    assert torch.equal(kernels.fp8_grouped_gemm(view, around[1:M + 1, 1:3], more.view(E4M3), scales, offsets), want)
+    # one group's rows beside another's: the neighbours in a tile are not multiplied into them either
+    two = torch.cat([a, torch.full((50, K), 0x7F, dtype=torch.uint8, device=cuda).view(E4M3)])
+    both = kernels.fp8_grouped_gemm(two, torch.cat([sa, torch.ones(50, 2, device=cuda)]), torch.cat([b, b]), torch.cat([sb, sb]),
+                                    torch.tensor([0, M, M + 50], dtype=torch.int32, device=cuda))
+    assert torch.equal(both[:M], want) and torch.isnan(both[M:]).all()
+
+
+def test_graph_of_a_product_over_every_kind_of_launch(cuda, lib):
+    """Captured once, replayed on other inputs: clusters, narrow and wide tiles, few rows."""
+    g = torch.Generator(device=cuda).manual_seed(12)
+    for M, N, K in ((1, 1024, 1024), (100, 512, 2048), (700, 640, 256), (2000, 4500, 256)):
+        a, sa, b, sb = _whole(M, N, K, 1, g, cuda)
+        kernels.fp8_gemm(a, sa, b[0], sb[0])
+        torch.cuda.synchronize(cuda)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = kernels.fp8_gemm(a, sa, b[0], sb[0], out_dtype=torch.float32)
+        for _ in range(2):
+            na, nsa, nb, nsb = _whole(M, N, K, 1, g, cuda)
+            for old, new in ((a, na), (sa, nsa), (b, nb), (sb, nsb)):
+                old.view(torch.uint8).copy_(new.view(torch.uint8)) if old.dtype == E4M3 else old.copy_(new)
+            graph.replay()
+            assert torch.equal(y, _product(na, nsa, nb[0], nsb[0])[0].float())

@@ -37,6 +37,18 @@ def test_quantize(no_library, x):
             call(x)
 
 
+def test_rows_whose_length_passes_31_bits(no_library):
+    """Their length would reach the library cut to 32 bits."""
+    long = torch.zeros(1).expand(2 ** 32 + 128)
+    for call in (lambda: kernels.fp8_quantize(long), lambda: kernels.fp8_silu_mul(long, long), lambda: kernels.fp8_quantize_blocks(long.view(1, -1)),
+                 lambda: kernels.fp8_quantize_blocks(torch.zeros(1, 1).expand(2 ** 32 + 1, 1))):
+        with pytest.raises(ValueError, match="more than"):
+            call()
+    byte = torch.zeros(1, 1).to(E4M3)
+    with pytest.raises(ValueError, match="none above"):
+        kernels.fp8_gemm(byte.expand(1, 2 ** 32), torch.ones(1, 1).expand(1, 2 ** 25), byte.expand(4, 2 ** 32), torch.ones(1, 1).expand(1, 2 ** 25))
+
+
 def test_blocks_need_rows(no_library):
     for x in (torch.zeros(128), torch.zeros(2, 0, 128)):
         with pytest.raises(ValueError):

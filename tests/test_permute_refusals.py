@@ -86,6 +86,8 @@ def test_c_entries(lib):
     assert lib.moe_permute(p, -16, 16, p, p, 4, 2, p, none) == -1
     assert lib.moe_permute(p, 16, 16, p, p, 1 << 30, 2, p, none) == -2
     assert lib.moe_permute(none, 16, 16, none, none, 0, 2, none, none) == 0
+    assert lib.moe_permute(p, 16, 16, p, p, 1 << 62, 8, p, none) == -2      # T * k would wrap around
+    assert lib.moe_unpermute(p, 8, p, p, none, 1 << 62, 8, 8, 0, p, none) == -2
     assert lib.moe_unpermute(p, 8, p, p, none, 4, 2, 8, 3, p, none) == -1
     assert lib.moe_unpermute(p, 8, p, none, none, 4, 2, 8, 0, p, none) == -1
     assert lib.moe_unpermute_grad(p, 8, none, 8, p, p, p, 4, 2, 8, 0, p, p, none) == -1

@@ -219,7 +219,7 @@ template <bool SWIGLU>
 static int quantize_rows(const void* x, int64_t x_stride, const void* up, int64_t up_stride, int64_t rows, int K, int dtype, void* q,
                          float* scale, const char* what, void* stream) {
   if (dtype < 0 || dtype > MOE_DTYPE_F32) return fail(MOE_ERR_ARG, "%s: unknown dtype %d", what, dtype);
-  if (rows < 0 || K < 1 || x_stride < 0 || up_stride < 0) return fail(MOE_ERR_ARG, "%s: bad shape rows=%lld K=%d", what, (long long)rows, K);
+  if (rows < 0 || K < 1 || K > 0x7FFF0000 || x_stride < 0 || up_stride < 0) return fail(MOE_ERR_ARG, "%s: bad shape rows=%lld K=%d", what, (long long)rows, K);
   if (rows == 0) return MOE_OK;
   const int64_t per_row = ceil_div64(K, G);
   if (rows > 0x7FFF0000ll / per_row) return fail(MOE_ERR_UNSUPPORTED, "%s: too many groups", what);
@@ -267,7 +267,7 @@ extern "C" int moe_fp8_quantize_blocks(const void* w, int64_t E, int64_t rows, i
   using namespace moe;
   using namespace moe::fp8;
   if (dtype < 0 || dtype > MOE_DTYPE_F32) return fail(MOE_ERR_ARG, "fp8_quantize_blocks: unknown dtype %d", dtype);
-  if (E < 0 || rows < 1 || K < 1) return fail(MOE_ERR_ARG, "fp8_quantize_blocks: bad shape %lld x %lld x %d", (long long)E, (long long)rows, K);
+  if (E < 0 || rows < 1 || K < 1 || K > 0x7FFF0000) return fail(MOE_ERR_ARG, "fp8_quantize_blocks: bad shape %lld x %lld x %d", (long long)E, (long long)rows, K);
   if (E == 0) return MOE_OK;
   if (!w || !q || !scale) return fail(MOE_ERR_ARG, "fp8_quantize_blocks: null pointer");
   const int64_t rb = ceil_div64(rows, G), cb = ceil_div64(K, G);

@@ -243,7 +243,7 @@ extern "C" int moe_permute(const void* src, int64_t src_stride, int64_t row_byte
   if (T < 0 || k < 1 || row_bytes < 1 || src_stride < 0) return fail(MOE_ERR_ARG, "permute: bad shape T=%lld k=%d row bytes=%lld stride=%lld", (long long)T, k, (long long)row_bytes, (long long)src_stride);
   if (T == 0) return MOE_OK;
   if (!src || !row_of || !live || !dst) return fail(MOE_ERR_ARG, "permute: null pointer");
-  if (T * k > 0x7FFFFFFFll || row_bytes > 0x7FFFFFFFll) return fail(MOE_ERR_UNSUPPORTED, "permute: too many rows or too wide ones");
+  if (T > 0x7FFFFFFFll || T * k > 0x7FFFFFFFll || row_bytes > 0x7FFF0000ll) return fail(MOE_ERR_UNSUPPORTED, "permute: too many rows or too wide ones");
   DeviceInfo dev;
   int rc = current_device_info(&dev);
   if (rc) return rc;
@@ -287,7 +287,7 @@ extern "C" int moe_unpermute(const void* rows, int64_t rows_stride, const int32_
   if (T < 0 || k < 1 || H < 1 || rows_stride < 0) return fail(MOE_ERR_ARG, "unpermute: bad shape T=%lld k=%d H=%lld", (long long)T, k, (long long)H);
   if (T == 0) return MOE_OK;
   if (!rows || !row_of || !live || !out) return fail(MOE_ERR_ARG, "unpermute: null pointer");
-  if (T * k > 0x7FFFFFFFll || H > 0x1FFFFFFFll) return fail(MOE_ERR_UNSUPPORTED, "unpermute: too many rows or too wide ones");
+  if (T > 0x7FFFFFFFll || T * k > 0x7FFFFFFFll || H > 0x1FFF0000ll) return fail(MOE_ERR_UNSUPPORTED, "unpermute: too many rows or too wide ones");
   DeviceInfo dev;
   int rc = current_device_info(&dev);
   if (rc) return rc;
@@ -329,7 +329,7 @@ extern "C" int moe_unpermute_grad(const void* gy, int64_t gy_stride, const void*
   if (T < 0 || k < 1 || H < 1 || gy_stride < 0 || rows_stride < 0) return fail(MOE_ERR_ARG, "unpermute_grad: bad shape T=%lld k=%d H=%lld", (long long)T, k, (long long)H);
   if (T == 0 || (!g_rows && !g_w)) return MOE_OK;
   if (!gy || !row_of || !live || !weights || (g_w && !rows)) return fail(MOE_ERR_ARG, "unpermute_grad: null pointer");
-  if (T * k > 0x7FFFFFFFll || H > 0x1FFFFFFFll) return fail(MOE_ERR_UNSUPPORTED, "unpermute_grad: too many rows or too wide ones");
+  if (T > 0x7FFFFFFFll || T * k > 0x7FFFFFFFll || H > 0x1FFF0000ll) return fail(MOE_ERR_UNSUPPORTED, "unpermute_grad: too many rows or too wide ones");
   DeviceInfo dev;
   int rc = current_device_info(&dev);
   if (rc) return rc;

@@ -17,6 +17,7 @@ import torch
 from . import _lib, ops
 
 GROUP = 128
+_WIDEST = 2 ** 31 - 2 ** 16       # the library counts the elements of a row in 32 bits
 E4M3 = torch.float8_e4m3fn
 _OUT_DTYPES = (None, torch.bfloat16, torch.float16, torch.float32)
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # MOE_DTYPE_* of include/moe_b200.h
@@ -42,6 +43,8 @@ def _input_type(x: torch.Tensor, least_dims: int) -> int:
         raise ValueError("8-bit values are made from bfloat16, float16 or float32")
     if x.dim() < least_dims or x.shape[-1] < 1 or (least_dims == 2 and x.shape[-2] < 1):
         raise ValueError(f"expected at least {least_dims} dimension(s), none of the last {least_dims} empty, got {tuple(x.shape)}")
+    if max(x.shape[-least_dims:]) > _WIDEST:
+        raise ValueError(f"rows of more than {_WIDEST} elements: cut them into groups of {GROUP} first")
     return _DTYPES[x.dtype]
 
 
@@ -106,8 +109,8 @@ def _product(a, a_scale, b, b_scale, E, offsets, out_dtype, out) -> torch.Tensor
     N, K2 = b.shape[-2:]
     if K2 != K:
         raise ValueError(f"inner dimensions differ: a has K={K}, b has K={K2}")
-    if K < 16 or K % 16 or N < 1 or E < 1:
-        raise ValueError(f"K={K} must be a positive multiple of 16, N={N} and E={E} positive")
+    if K < 16 or K % 16 or N < 1 or E < 1 or max(K, N) > _WIDEST:
+        raise ValueError(f"K={K} must be a positive multiple of 16, N={N} and E={E} positive, none above {_WIDEST}")
     kb, nb = _groups(K), _groups(N)
     if a_scale.dtype != torch.float32 or a_scale.shape != (M, kb):
         raise ValueError(f"a_scale must be float32 [{M}, {kb}]")

@@ -20,7 +20,7 @@ from . import _lib, ops
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # MOE_DTYPE_* of include/moe_b200.h
 
 
-@dataclass(frozen=True)
+@dataclass(frozen=True, eq=False)
 class MoESort:
     """Tables of one routing: contiguous int32 tensors on one device, usable by any number of permutes and unpermutes."""
     offsets: torch.Tensor    # [E + 1]: first row of every expert; offsets[E] rows hold an entry
