@@ -324,6 +324,10 @@ __device__ __forceinline__ void zero_rows(const Params& p, int64_t ahead, int64_
   for (int64_t i = w; i < ahead + p.rows - behind; i += n) {
     const int64_t r = i < ahead ? i : behind + i - ahead;
     unsigned char* y = reinterpret_cast<unsigned char*>(p.Y) + r * p.ldy * (p.out == MOE_DTYPE_F32 ? 4 : 2);
+    if (p.vec_store) {
+      for (int c = lane; c < (p.out == MOE_DTYPE_F32 ? p.N / 4 : p.N / 8); c += 32) reinterpret_cast<uint4*>(y)[c] = make_uint4(0u, 0u, 0u, 0u);
+      continue;
+    }
     for (int c = lane; c < p.N; c += 32) {
       if (p.out == MOE_DTYPE_F32) reinterpret_cast<uint32_t*>(y)[c] = 0u;
       else reinterpret_cast<uint16_t*>(y)[c] = 0;

@@ -221,6 +221,9 @@ static unsigned grid_for(int64_t items, int64_t per_cta, int64_t cap) {
   return (unsigned)(b < 1 ? 1 : (b > cap ? cap : b));
 }
 
+// CTAs that an SM can hold, for kernels that walk over the tokens: rows of few vectors make small ones
+static int64_t resident(int sms, unsigned threads) { return (int64_t)sms * (threads >= 64 ? 2048 / threads : 32); }
+
 }  // namespace perm
 }  // namespace moe
 
@@ -271,7 +274,7 @@ static void launch_unpermute(const void* rows, int64_t stride, const int32_t* ro
                              int k, int64_t H, void* out, int sms, cudaStream_t st) {
   using namespace moe::perm;
   const int vecs = (int)(H * sizeof(T) / V);
-  const unsigned grid = grid_for(tokens, 1, (int64_t)sms * 8), threads = threads_for(vecs, V);
+  const unsigned threads = threads_for(vecs, V), grid = grid_for(tokens, 1, resident(sms, threads));
   const T* r = reinterpret_cast<const T*>(rows);
   T* o = reinterpret_cast<T*>(out);
   if (k <= 4) unpermute_kernel<T, V, true, 4><<<grid, threads, 0, st>>>(r, stride, row_of, live, w, tokens, k, vecs, o);
@@ -316,7 +319,7 @@ static void launch_unpermute_grad(const void* gy, int64_t gy_stride, const void*
   const T *g = reinterpret_cast<const T*>(gy), *r = reinterpret_cast<const T*>(rows);
   T* gr = reinterpret_cast<T*>(g_rows);
   const int64_t items = tokens * ((k + GRAD_SLOTS - 1) / GRAD_SLOTS);
-  unpermute_grad_kernel<T, V><<<grid_for(items, 1, (int64_t)sms * 8), threads, 0, st>>>(g, gy_stride, r, rows_stride, row_of, live, w, tokens, k,
+  unpermute_grad_kernel<T, V><<<grid_for(items, 1, resident(sms, threads)), threads, 0, st>>>(g, gy_stride, r, rows_stride, row_of, live, w, tokens, k,
                                                                                      vecs, gr, g_w);
 }
 
