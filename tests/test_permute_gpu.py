@@ -43,7 +43,7 @@ def _tables(ids, E):
 
 
 @pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
-@pytest.mark.parametrize("T,k,E", [(1, 1, 1), (1, 8, 3), (7, 2, 5), (300, 8, 17), (5000, 2, 64), (1, 40, 2), (40000, 2, 1200)])
+@pytest.mark.parametrize("T,k,E", [(1, 1, 1), (1, 8, 3), (7, 2, 5), (300, 8, 17), (5000, 2, 64), (1, 40, 2), (40000, 2, 1200), (500, 3, 5119), (70000, 1, 100)])
 def test_sort(cuda, lib, T, k, E, dtype):
     g = torch.Generator().manual_seed(T + k)
     ids = _ids(T, k, E, g, dtype=dtype)

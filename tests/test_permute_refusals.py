@@ -34,7 +34,8 @@ def test_cpu_tensors_are_rejected():
 
 
 @pytest.mark.parametrize("ids,E", [(torch.zeros(4, 2), 3), (torch.zeros(4, 2, dtype=torch.int16), 3), (torch.zeros(4, 2, 1, dtype=torch.int32), 3),
-                                   (torch.zeros(4, 0, dtype=torch.int32), 3), (torch.zeros(4, 2, dtype=torch.int32), 0)])
+                                   (torch.zeros(4, 0, dtype=torch.int32), 3), (torch.zeros(4, 2, dtype=torch.int32), 0), (torch.zeros(4, 2, dtype=torch.int32), 5120),
+                                   (torch.zeros(4, 2, dtype=torch.int32), 2 ** 33)])
 def test_sort(no_library, ids, E):
     with pytest.raises(ValueError):
         kernels.moe_sort(ids, E)
@@ -80,6 +81,7 @@ def test_c_entries(lib):
     assert lib.moe_sort(p, 0, 4, 0, p, p, p, p, p, 1 << 20, none) == -1
     assert lib.moe_sort(p, 0, 4, 3, p, p, none, p, p, 1 << 20, none) == -1
     assert lib.moe_sort(p, 0, 4, 3, p, p, p, p, none, 0, none) == -3
+    assert lib.moe_sort(p, 0, 4, 5120, p, p, p, p, p, 1 << 20, none) == -2 and lib.moe_sort(p, 0, 4, 5119, p, p, p, p, none, 0, none) == -3
     assert lib.moe_sort(p, 0, 4, 8000, p, p, p, p, p, 1 << 20, none) == -2 and b"too large" in lib.moe_last_error()
     assert lib.moe_permute(none, 16, 16, p, p, 4, 2, p, none) == -1
     assert lib.moe_permute(p, 16, 0, p, p, 4, 2, p, none) == -1

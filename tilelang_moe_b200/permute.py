@@ -17,6 +17,7 @@ import torch
 
 from . import _lib, ops
 
+_MAX_EXPERTS = 5119        # groups that the library's counting kernel has shared memory for, but the one of no expert
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # MOE_DTYPE_* of include/moe_b200.h
 
 
@@ -62,19 +63,18 @@ def moe_sort(topk_ids: torch.Tensor, n_experts: int) -> MoESort:
         raise ValueError("expert ids must be int64 or int32")
     if topk_ids.dim() not in (1, 2) or (topk_ids.dim() == 2 and topk_ids.shape[1] < 1):
         raise ValueError("expert ids must be [T] or [T, k]")
-    if n_experts < 1:
-        raise ValueError(f"n_experts={n_experts} must be positive")
+    if not 1 <= n_experts <= _MAX_EXPERTS:
+        raise ValueError(f"n_experts={n_experts} must be in [1, {_MAX_EXPERTS}]")
     ids = topk_ids.contiguous()
     n, dev = ids.numel(), ids.device
     lib = _lib.load()
-    # one allocation: counts [E + 1], offsets [E + 2], perm [n], row_of [n]
-    buf = torch.empty(2 * n_experts + 3 + 2 * n, dtype=torch.int32, device=dev)
-    _, offsets, _, perm, row_of = buf.split_with_sizes((n_experts + 1, n_experts + 1, 1, n, n))
+    # one allocation: counts [E + 1], offsets [E + 2], perm [n], row_of [n] and the scratch of the call
     need = lib.moe_sort_workspace(n, n_experts)
-    ws = torch.empty(max(need, 4), dtype=torch.uint8, device=dev)
+    buf = torch.empty(2 * n_experts + 3 + 2 * n + (need + 3) // 4, dtype=torch.int32, device=dev)
+    _, offsets, _, perm, row_of, ws = buf.split_with_sizes((n_experts + 1, n_experts + 1, 1, n, n, (need + 3) // 4))
     with ops._on(dev):
-        rc = lib.moe_sort(ops._ptr(ids), int(ids.dtype == torch.int64), n, n_experts, ops._ptr(buf), ops._ptr(offsets),
-                          ops._ptr(perm), ops._ptr(row_of), ops._ptr(ws), need, ops._stream())
+        rc = lib.moe_sort(ids.data_ptr(), int(ids.dtype == torch.int64), n, n_experts, buf.data_ptr(), offsets.data_ptr(),
+                          perm.data_ptr(), row_of.data_ptr(), ws.data_ptr(), need, ops._stream())
     _lib.check(rc, "moe_sort")
     ops._after(dev)
     return MoESort._of(offsets, perm, row_of, ids.shape[1] if ids.dim() == 2 else 1)
