@@ -8,8 +8,8 @@
 //   g_rows[row_of[t,j], :] = w[t,j] * gy[t, :]        g_w[t,j] = <rows[row_of[t,j], :], gy[t, :]>
 //
 // All of it is bound by memory.  Every kernel goes by tokens, not by sorted rows: a token's row is read once and written to
-// its k places (permute, gradient of unpermute), or its k rows are read and leave as one (unpermute), so nothing is read
-// twice and no sum needs an atomic; the order of every sum is fixed.
+// its k places (permute; the gradient of unpermute reads it once for every four of them), or its k rows are read and leave as
+// one (unpermute), so no row is read for every copy of it and no sum needs an atomic; the order of every sum is fixed.
 #include "vec.cuh"
 
 namespace moe {
