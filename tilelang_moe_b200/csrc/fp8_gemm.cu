@@ -142,6 +142,26 @@ __device__ __forceinline__ float2 unpair(f32x2 v) {
   return r;
 }
 __device__ __forceinline__ void fma2(f32x2& acc, f32x2 v, f32x2 s) { asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s)); }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ bool no_normal_number(float s) { return (__float_as_uint(s) << 1) - 0x01000000u >= 0xFE000000u; }
+// A block's sum times both of its scales: (sum * pre) * post.  Their product alone serves, and pre is 1, while it is a normal
+// number.  Where two finite scales leave that range the sum meets the larger one first if their product is too small, the smaller
+// one first if it is too large, so that what is rounded in between is no further from the result's range than the result.  A
+// row's bits do not depend on which way its neighbours in the warp go: times 1 is exact.
+__device__ __forceinline__ void split_scale(float a, float b, float& pre, float& post) {
+  const float s = a * b, big = fmaxf(fabsf(a), fabsf(b));
+  pre = 1.0f;
+  post = s;
+  if (!no_normal_number(s) || a == 0.0f || b == 0.0f || !(big <= 0x1.fffffep127f)) return;    // zero and infinity stay what they are
+  const bool a_first = (fabsf(s) < 1.0f) == (fabsf(a) == big);
+  pre = a_first ? a : b;
+  post = a_first ? b : a;
+}
 
 // The wait of the accumulating warps, without the call of mbar_wait: around a call every register is spoken for.
 __device__ __forceinline__ bool mbar_wait_inline(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int site) {
@@ -475,6 +495,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
       float a_next = *sa, b_next = *sb;
       for (int kb = kb0; kb < kb1; ++kb) {
         const float s = a_next * b_next;
+        const bool far = __any_sync(0xFFFFFFFFu, no_normal_number(s)) && any_row;
         if (kb + 1 < kb1) {
           sa += p.sa_k;
           ++sb;
@@ -484,8 +505,22 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__
         if (!mbar_wait_inline(tfull0 + 8 * buf, buf_phase, abort_flag, p.status, 34)) { ok = false; break; }
         tc_fence_after();
         const uint32_t taddr = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(buf * BN + half * COLS);
-        const f32x2 s2 = pair_of(s, s);
-        if (any_row) {
+        if (far) {
+          // Read again: keeping both scales would cost every block two registers.  8192 x 4096 x 7168 us: no check 228.4, with it 231.7,
+          // every block here (scales of zero come here too) 285.  The product applied to tensor memory in place instead of this
+          // second form of the additions: 242 to 264 for ordinary blocks.
+          float pre, post;
+          split_scale(kb + 1 < kb1 ? *(sa - p.sa_k) : *sa, kb + 1 < kb1 ? *(sb - 1) : *sb, pre, post);
+          const f32x2 pre2 = pair_of(pre, pre), post2 = pair_of(post, post);
+#pragma unroll
+          for (int c = 0; c < COLS / 16; ++c) {
+            f32x2 v[8];
+            tmem_ld16_pairs(taddr + c * 16, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) fma2(acc[c * 8 + j], mul2(v[j], pre2), post2);
+          }
+        } else if (any_row) {
+          const f32x2 s2 = pair_of(s, s);
 #pragma unroll
           for (int c = 0; c < COLS / 16; ++c) {
             f32x2 v[8];
