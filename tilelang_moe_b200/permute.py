@@ -23,7 +23,8 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # MOE_DTYPE_
 
 @dataclass(frozen=True, eq=False)
 class MoESort:
-    """Tables of one routing: contiguous int32 tensors on one device, usable by any number of permutes and unpermutes."""
+    """Tables of one routing: contiguous int32 tensors on one device, usable by any number of permutes and unpermutes.  A backward
+    pass reads offsets and row_of again: it raises where they have been written to in between."""
     offsets: torch.Tensor    # [E + 1]: first row of every expert; offsets[E] rows hold an entry
     perm: torch.Tensor       # [T * k]: entry t * k + j at each sorted row
     row_of: torch.Tensor     # [T * k]: sorted row of each entry
@@ -137,34 +138,47 @@ def _unpermute_grad(gy: torch.Tensor, rows: Optional[torch.Tensor], sort: MoESor
     return g_rows, g_w
 
 
+def _keep(ctx, sort: MoESort, *others) -> None:
+    """Saves what the backward pass reads of the tables, under autograd's eyes: written again before it, they raise there.
+    Tables of inference mode cannot be watched: of those the step keeps a copy."""
+    tables = (t.clone() if t.is_inference() else t for t in (sort.offsets, sort.row_of))
+    ctx.k = sort.k
+    ctx.save_for_backward(*tables, *others)
+
+
+def _kept(ctx):
+    offsets, row_of, *others = ctx.saved_tensors
+    return (MoESort._of(offsets, None, row_of, ctx.k), *others)
+
+
 class _Permute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, sort):
-        ctx.sort = sort
+        _keep(ctx, sort)
         return _permute(x, sort)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        return _unpermute(g, ctx.sort, None), None
+        sort, = _kept(ctx)
+        return _unpermute(g, sort, None), None
 
 
 class _Unpermute(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, sort):
-        ctx.sort = sort
         rows = _rows(rows)
         # the rows are only kept where the weights' gradient needs them
-        ctx.save_for_backward(rows if weights is not None and ctx.needs_input_grad[1] else None, weights)
+        _keep(ctx, sort, rows if weights is not None and ctx.needs_input_grad[1] else None, weights)
         return _unpermute(rows, sort, weights)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
-        rows, weights = ctx.saved_tensors
+        sort, rows, weights = _kept(ctx)
         if weights is None:
-            return _permute(gy, ctx.sort), None, None
-        return (*_unpermute_grad(gy, rows, ctx.sort, weights, ctx.needs_input_grad[0], ctx.needs_input_grad[1]), None)
+            return _permute(gy, sort), None, None
+        return (*_unpermute_grad(gy, rows, sort, weights, ctx.needs_input_grad[0], ctx.needs_input_grad[1]), None)
 
 
 def moe_permute(x: torch.Tensor, sort: MoESort) -> torch.Tensor:
