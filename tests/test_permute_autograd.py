@@ -137,3 +137,34 @@ def test_tables_made_in_inference_mode(on_host):
         sort.row_of.copy_(_sort(OTHER, E).row_of)
     for a, b in zip(torch.autograd.grad(y, (x, w), gy), torch.autograd.grad(_formula(IDS, x, w, scale), (x, w), gy.double())):
         assert torch.allclose(a, b.float(), rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("call", ["permute", "rows", "weights"])
+def test_forward_mode_is_refused(on_host, call, grad):
+    """Without a rule for it the tangent would be lost, which reads as a derivative of zero."""
+    sort = _sort(IDS, E)
+    x, rows, w = torch.randn(T, H), torch.randn(T * K, H), torch.rand(T, K)
+    with torch.set_grad_enabled(grad), torch.autograd.forward_ad.dual_level():
+        def dual(t):
+            return torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            if call == "permute":
+                kernels.moe_permute(dual(x), sort)
+            elif call == "rows":
+                kernels.moe_unpermute(dual(rows), sort, w)
+            else:
+                kernels.moe_unpermute(rows, sort, dual(w))
+        # what has no tangent is computed there as anywhere else
+        assert torch.equal(kernels.moe_unpermute(kernels.moe_permute(x, sort), sort, w).detach(), _loss(sort, x, w, 1.0).detach())
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(lambda t: kernels.moe_permute(t, sort), (x,), (torch.ones_like(x),))
+
+
+def test_gradients_of_gradients_are_refused(on_host):
+    x, w, scale, gy = _operands()
+    y = _loss(_sort(IDS, E), x, w, scale)
+    gx, = torch.autograd.grad(y, x, gy.requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError):
+        gx.sum().backward()

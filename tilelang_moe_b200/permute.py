@@ -6,7 +6,8 @@
 
 Rows sort.offsets[e] .. sort.offsets[e+1] - 1 belong to expert e.  An id outside [0, n_experts) marks an entry without an
 expert (a padded token, an entry over an expert's capacity): its row lies behind offsets[n_experts], holds zeros, and adds
-nothing; its gradients are zero.  Results and gradients are computed without atomics, in a fixed order.
+nothing; its gradients are zero.  Results and gradients are computed without atomics, in a fixed order.  Gradients are those of
+the backward pass; forward mode is refused.
 """
 from __future__ import annotations
 
@@ -14,6 +15,7 @@ from dataclasses import dataclass
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib, ops
 
@@ -181,6 +183,12 @@ class _Unpermute(torch.autograd.Function):
         return (*_unpermute_grad(gy, rows, sort, weights, ctx.needs_input_grad[0], ctx.needs_input_grad[1]), None)
 
 
+def _forward_mode() -> bool:
+    """Inside a forward-mode level a tensor may carry a tangent.  There the calls go through autograd, which refuses those that do:
+    past it the tangent would be lost without a word."""
+    return forward_ad._current_level >= 0
+
+
 def moe_permute(x: torch.Tensor, sort: MoESort) -> torch.Tensor:
     """Rows of x [T, H] at their entries' places: [T*k, H] of x's type.  Any element type; floating types of 16 and 32 bits
     have a gradient, others (8-bit values beside their scales, say) are copied."""
@@ -189,11 +197,10 @@ def moe_permute(x: torch.Tensor, sort: MoESort) -> torch.Tensor:
         raise ValueError(f"x must be [{sort.tokens}, H], one row for each token of the sort")
     if x.device != sort.row_of.device:
         raise ValueError(f"x is on {x.device}, the sort's tables on {sort.row_of.device}")
-    if x.requires_grad and torch.is_grad_enabled():
-        if x.dtype not in _DTYPES:
-            raise ValueError("the gradient of moe_permute is computed in bfloat16, float16 or float32")
-        return _Permute.apply(x, sort)
-    return _permute(x, sort)
+    backward = x.requires_grad and torch.is_grad_enabled()
+    if backward and x.dtype not in _DTYPES:
+        raise ValueError("the gradient of moe_permute is computed in bfloat16, float16 or float32")
+    return _Permute.apply(x, sort) if backward or _forward_mode() else _permute(x, sort)
 
 
 def moe_unpermute(rows: torch.Tensor, sort: MoESort, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -211,6 +218,6 @@ def moe_unpermute(rows: torch.Tensor, sort: MoESort, weights: Optional[torch.Ten
         if weights.dtype != torch.float32 or weights.shape != (n // k, k):
             raise ValueError(f"routing weights must be float32 [{n // k}, {k}]")
         weights = weights.contiguous()
-    if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
+    if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)) or _forward_mode():
         return _Unpermute.apply(rows, weights, sort)
     return _unpermute(rows, sort, weights)
