@@ -29,6 +29,7 @@ def _groups(n: int) -> int:
 
 def _rows2(x: torch.Tensor) -> torch.Tensor:
     """x [..., K] as a matrix of packed rows at one non-negative stride; a copy where its strides do not allow that."""
+    x = ops._carried_out(x)
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1])
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
@@ -87,7 +88,7 @@ def fp8_quantize_blocks(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """w [..., N, K] -> (e4m3 [..., N, K], scale float32 [..., ceil(N / 128), ceil(K / 128)])."""
     ops._need_cuda(w)
     dt = _input_type(w, 2)
-    w = w.contiguous()
+    w = ops._carried_out(w).contiguous()
     N, K = w.shape[-2:]
     q = torch.empty(w.shape, dtype=E4M3, device=w.device)
     scale = torch.empty(*w.shape[:-2], _groups(N), _groups(K), dtype=torch.float32, device=w.device)
@@ -132,6 +133,8 @@ def _product(a, a_scale, b, b_scale, E, offsets, out_dtype, out) -> torch.Tensor
     else:
         if out.shape != (M, N) or out.dtype not in _DTYPES or (M > 0 and N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise ValueError(f"out must be [{M}, {N}] in bfloat16, float16 or float32 with packed rows that do not overlap")
+        if out.is_neg():
+            raise ValueError("out is the negative of what its memory holds")
         if out_dtype is not None and out_dtype != out.dtype:
             raise ValueError(f"out is {out.dtype}, not {out_dtype}")
     lda = _stride(a)
@@ -140,7 +143,7 @@ def _product(a, a_scale, b, b_scale, E, offsets, out_dtype, out) -> torch.Tensor
         lda = K
     if not b.is_contiguous() or b.data_ptr() & 15:
         b = b.clone(memory_format=torch.contiguous_format)
-    b_scale = b_scale.contiguous()
+    a_scale, b_scale = ops._carried_out(a_scale), ops._carried_out(b_scale).contiguous()
     lib = _lib.load()
     with ops._on(dev):
         rc = lib.moe_fp8_gemm(a.data_ptr(), lda, a_scale.data_ptr(), *a_scale.stride(), b.data_ptr(), b_scale.data_ptr(),

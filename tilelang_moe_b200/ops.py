@@ -66,6 +66,11 @@ def _need_cuda(*ts: torch.Tensor) -> None:
             raise ValueError("moe_b200 operates on CUDA tensors only (no CPU path)")
 
 
+def _carried_out(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy where it is a conjugate or negative that its memory does not hold yet."""
+    return t.resolve_conj().resolve_neg() if t.is_neg() or t.is_conj() else t
+
+
 def status_buffer(device: torch.device) -> torch.Tensor:
     key = device.index if isinstance(device, torch.device) else torch.device(device).index
     if key is None:

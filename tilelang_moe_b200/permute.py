@@ -85,6 +85,7 @@ def moe_sort(topk_ids: torch.Tensor, n_experts: int) -> MoESort:
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t with packed rows at any non-negative stride."""
+    t = ops._carried_out(t)
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -217,7 +218,7 @@ def moe_unpermute(rows: torch.Tensor, sort: MoESort, weights: Optional[torch.Ten
     if weights is not None:
         if weights.dtype != torch.float32 or weights.shape != (n // k, k):
             raise ValueError(f"routing weights must be float32 [{n // k}, {k}]")
-        weights = weights.contiguous()
+        weights = ops._carried_out(weights).contiguous()
     if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)) or _forward_mode():
         return _Unpermute.apply(rows, weights, sort)
     return _unpermute(rows, sort, weights)
