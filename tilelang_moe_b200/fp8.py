@@ -133,6 +133,8 @@ def _product(a, a_scale, b, b_scale, E, offsets, out_dtype, out) -> torch.Tensor
     else:
         if out.shape != (M, N) or out.dtype not in _DTYPES or (M > 0 and N > 1 and out.stride(1) != 1) or (M > 1 and out.stride(0) < N):
             raise ValueError(f"out must be [{M}, {N}] in bfloat16, float16 or float32 with packed rows that do not overlap")
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("out requires a gradient, and these products have none")
         if out.is_neg():
             raise ValueError("out is the negative of what its memory holds")
         if out_dtype is not None and out_dtype != out.dtype:
@@ -150,6 +152,8 @@ def _product(a, a_scale, b, b_scale, E, offsets, out_dtype, out) -> torch.Tensor
                               ops._ptr(offsets), M, K, N, E, out.data_ptr(), N if fresh else _stride(out), _DTYPES[out.dtype], int(fresh),
                               ops.status_buffer(dev).data_ptr(), ops._stream())
     _lib.check(rc, "moe_fp8_gemm")
+    if not fresh:
+        torch.autograd.graph.increment_version(out)      # what autograd has saved of it is no longer there
     ops._after(dev)
     return out
 
