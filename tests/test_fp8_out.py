@@ -66,3 +66,15 @@ def test_a_tensor_of_inference_mode():
         out = torch.ones(4, 8)
         assert _gemm(out) is out
     assert _gemm(out) is out
+
+
+def test_more_experts_than_the_library_takes():
+    """Refused as every other bad shape is, before the library is asked; 1024 are taken."""
+    for E, taken in ((1024, True), (1025, False), (5119, False)):
+        args = (torch.zeros(4, 16).to(E4M3), torch.ones(4, 1), torch.zeros(E, 1, 16).to(E4M3), torch.ones(E, 1, 1), torch.zeros(E + 1).int())
+        if taken:
+            kernels.fp8_grouped_gemm(*args)
+        else:
+            with pytest.raises(ValueError, match="1024"):
+                kernels.fp8_grouped_gemm(*args)
+    assert _Library.calls == 1

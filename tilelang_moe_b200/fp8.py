@@ -18,6 +18,7 @@ from . import _lib, ops
 
 GROUP = 128
 _WIDEST = 2 ** 31 - 2 ** 16       # the library counts the elements of a row in 32 bits
+_MAX_EXPERTS = 1024               # the product keeps its table of groups in shared memory
 E4M3 = torch.float8_e4m3fn
 _OUT_DTYPES = (None, torch.bfloat16, torch.float16, torch.float32)
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # MOE_DTYPE_* of include/moe_b200.h
@@ -112,6 +113,8 @@ def _product(a, a_scale, b, b_scale, E, offsets, out_dtype, out) -> torch.Tensor
         raise ValueError(f"inner dimensions differ: a has K={K}, b has K={K2}")
     if K < 16 or K % 16 or N < 1 or E < 1 or max(K, N) > _WIDEST:
         raise ValueError(f"K={K} must be a positive multiple of 16, N={N} and E={E} positive, none above {_WIDEST}")
+    if E > _MAX_EXPERTS:
+        raise ValueError(f"E={E} exceeds the {_MAX_EXPERTS} experts of one product")
     kb, nb = _groups(K), _groups(N)
     if a_scale.dtype != torch.float32 or a_scale.shape != (M, kb):
         raise ValueError(f"a_scale must be float32 [{M}, {kb}]")
@@ -171,8 +174,8 @@ def fp8_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: t
 def fp8_grouped_gemm(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor, offsets: torch.Tensor,
                      out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[r] = fp8_gemm with b[e] for the rows offsets[e] .. offsets[e + 1] - 1 of every expert e: b e4m3 [E, N, K] with b_scale
-    float32 [E, ceil(N / 128), ceil(K / 128)], offsets int32 [E + 1] on the device (no host synchronisation).  Rows of no
-    expert (behind offsets[E]) are zero in a new tensor and left as they were in ``out``."""
+    float32 [E, ceil(N / 128), ceil(K / 128)], offsets int32 [E + 1] on the device (no host synchronisation); E at most 1024, where
+    moe_sort takes 5119.  Rows of no expert (behind offsets[E]) are zero in a new tensor and left as they were in ``out``."""
     if offsets is None or b.dim() != 3:
         raise ValueError("b must be [E, N, K] and offsets int32 [E + 1]")
     return _product(a, a_scale, b, b_scale, b.shape[0], offsets, out_dtype, out)
