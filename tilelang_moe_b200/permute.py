@@ -20,6 +20,7 @@ from torch.autograd import forward_ad
 from . import _lib, ops
 
 _MAX_EXPERTS = 5119        # groups that the library's counting kernel has shared memory for, but the one of no expert
+_SCRATCH_KEPT = 4096       # bytes of scratch that a sort may keep beside its tables: an allocation less in a step of few tokens
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # MOE_DTYPE_* of include/moe_b200.h
 
 
@@ -71,10 +72,14 @@ def moe_sort(topk_ids: torch.Tensor, n_experts: int) -> MoESort:
     ids = topk_ids.contiguous()
     n, dev = ids.numel(), ids.device
     lib = _lib.load()
-    # one allocation: counts [E + 1], offsets [E + 2], perm [n], row_of [n] and the scratch of the call
+    # One allocation: counts [E + 1], offsets [E + 2], perm [n], row_of [n], and the scratch of the call where that is little.  More of
+    # it goes when the call returns: the tables live until the backward pass.
     need = lib.moe_sort_workspace(n, n_experts)
-    buf = torch.empty(2 * n_experts + 3 + 2 * n + (need + 3) // 4, dtype=torch.int32, device=dev)
-    _, offsets, _, perm, row_of, ws = buf.split_with_sizes((n_experts + 1, n_experts + 1, 1, n, n, (need + 3) // 4))
+    with_tables = (need + 3) // 4 if need <= _SCRATCH_KEPT else 0
+    buf = torch.empty(2 * n_experts + 3 + 2 * n + with_tables, dtype=torch.int32, device=dev)
+    _, offsets, _, perm, row_of, ws = buf.split_with_sizes((n_experts + 1, n_experts + 1, 1, n, n, with_tables))
+    if need > _SCRATCH_KEPT:
+        ws = torch.empty((need + 3) // 4, dtype=torch.int32, device=dev)
     with ops._on(dev):
         rc = lib.moe_sort(ids.data_ptr(), int(ids.dtype == torch.int64), n, n_experts, buf.data_ptr(), offsets.data_ptr(),
                           perm.data_ptr(), row_of.data_ptr(), ws.data_ptr(), need, ops._stream())
