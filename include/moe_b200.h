@@ -187,7 +187,7 @@ int moe_fp8_quantize_blocks(const void* w, int64_t E, int64_t rows, int K, int d
  *   Y        MOE_DTYPE_BF16 / F16 / F32 [rows, N], row stride ldy (elements).  Rows of no
  *            group are left as they were, or set to zero where zero_tail != 0
  * Products and sums in fp32, one rounding to the output type; the product of two scales may leave the range of fp32
- * where the term does not.  E <= 1024.
+ * where the term does not.  E <= 1024; K and N <= 0x7FFF0000.
  */
 int moe_fp8_gemm(const void* A, int64_t lda, const float* a_scale, int64_t as_row, int64_t as_k, const void* B,
                  const float* b_scale, const int32_t* offsets, int64_t rows, int K, int N, int E, void* Y, int64_t ldy,

@@ -643,6 +643,7 @@ extern "C" int moe_fp8_gemm(const void* A, int64_t lda, const float* a_scale, in
   if (out_dtype < 0 || out_dtype > MOE_DTYPE_F32) return fail(MOE_ERR_ARG, "fp8_gemm: unknown output type %d", out_dtype);
   if (rows < 0 || K < 16 || K % 16 || N < 1 || E < 1)
     return fail(MOE_ERR_ARG, "fp8_gemm: bad shape rows=%lld K=%d N=%d E=%d (K a multiple of 16)", (long long)rows, K, N, E);
+  if (K > 0x7FFF0000 || N > 0x7FFF0000) return fail(MOE_ERR_UNSUPPORTED, "fp8_gemm: K=%d or N=%d too wide", K, N);
   if (E > MAX_E) return fail(MOE_ERR_UNSUPPORTED, "fp8_gemm: E=%d exceeds %d", E, MAX_E);
   if (!offsets && E != 1) return fail(MOE_ERR_ARG, "fp8_gemm: several groups need an offsets table");
   if (rows == 0) return MOE_OK;

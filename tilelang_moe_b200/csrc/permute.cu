@@ -228,12 +228,15 @@ static int64_t resident(int sms, unsigned threads) { return (int64_t)sms * (thre
 }  // namespace moe
 
 // ====================================================================================
-extern "C" size_t moe_sort_workspace(int64_t n, int E) { return moe_route_histogram_workspace(n, E + 1); }
+// one group more than experts; no number of them that the histogram takes is anywhere near the largest int
+constexpr int SORT_MAX_E = 1 << 30;
+extern "C" size_t moe_sort_workspace(int64_t n, int E) { return E < 1 || E > SORT_MAX_E ? 0 : moe_route_histogram_workspace(n, E + 1); }
 
 extern "C" int moe_sort(const void* ids, int idx_is_int64, int64_t n, int E, int32_t* counts, int32_t* offsets, int32_t* perm,
                         int32_t* row_of, void* ws, size_t ws_bytes, void* stream) {
   using namespace moe;
   if (E < 1) return fail(MOE_ERR_ARG, "sort: bad expert count %d", E);
+  if (E > SORT_MAX_E) return fail(MOE_ERR_UNSUPPORTED, "sort: E=%d too large", E);
   if (n > 0 && (!perm || !row_of)) return fail(MOE_ERR_ARG, "sort: null perm/row_of");
   return route_histogram_ex(ids, idx_is_int64, n, E + 1, nullptr, counts, offsets, perm, row_of, ws, ws_bytes, nullptr, stream,
                             ROUTE_KEEP_ALL, false);
