@@ -16,10 +16,6 @@ template <> struct RawOf<2> { using type = uint16_t; };
 template <> struct RawOf<1> { using type = uint8_t; };
 template <int V> using Raw = typename RawOf<V>::type;
 
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-
 template <class T> __device__ __forceinline__ float2 halves(uint32_t w);
 template <> __device__ __forceinline__ float2 halves<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 template <> __device__ __forceinline__ float2 halves<__nv_bfloat16>(uint32_t w) {
