@@ -29,13 +29,13 @@ def on_host(monkeypatch):
 
 
 @pytest.mark.parametrize("T,k,E", [(1, 1, 1), (8, 2, 8), (2000, 8, 256), (0, 4, 3), (999, 3, 5119)])
-@pytest.mark.parametrize("need", [0, 2, 36, 4096, 4097, 1 << 20])
+@pytest.mark.parametrize("need", [0, 2, 36, 4097, 65536, 65537, 1 << 20])
 def test_scratch_does_not_outlive_the_call(monkeypatch, T, k, E, need):
     monkeypatch.setattr(_Library, "need", need)
     sort = kernels.moe_sort(torch.zeros(T, k, dtype=torch.int32), E)
     tables = 4 * (E + 1) + 4 * (E + 2) + 2 * 4 * T * k
     kept = {t.untyped_storage().data_ptr(): t.untyped_storage().nbytes() for t in (sort.offsets, sort.perm, sort.row_of)}
-    assert sum(kept.values()) <= tables + 4096
+    assert sum(kept.values()) <= tables + 65536
     at = _Library.seen
     assert at["offsets"][0] == sort.offsets.data_ptr() and at["ws"][1] == need
     assert T == 0 or (at["perm"][0], at["row_of"][0]) == (sort.perm.data_ptr(), sort.row_of.data_ptr())

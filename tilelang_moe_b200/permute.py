@@ -20,7 +20,9 @@ from torch.autograd import forward_ad
 from . import _lib, ops
 
 _MAX_EXPERTS = 5119        # groups that the library's counting kernel has shared memory for, but the one of no expert
-_SCRATCH_KEPT = 4096       # bytes of scratch that a sort may keep beside its tables: an allocation less in a step of few tokens
+# Bytes of scratch that a sort may keep beside its tables.  An allocation of its own costs a call 1.9 of 15 us, which counts in a step
+# of few tokens; a training step's scratch (16000 entries of 256 experts: 125 KB) would double what lives until the backward pass.
+_SCRATCH_KEPT = 64 * 1024
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}   # MOE_DTYPE_* of include/moe_b200.h
 
 
