@@ -12,11 +12,14 @@
 //   warps 2..9  one tile row and half of the tile's columns per thread: acc += (sa * sb) * block sum, while the other
 //               accumulator is being filled; after the last block convert and store.
 //
-// What bounds it.  Many rows: the power cap.  8192 x 4096 x 7168 takes 231 us from idle and 269 back to back (2.08 and 1.79 PFLOP/s)
-// with the clocks at 1.45 to 1.5 GHz and 1000 W; the library's product without block scales 167 and 200.  An accumulating warp
-// needs about 500 of the 870 clocks of a k-block.  A form on CTA pairs (cta_group::2, two thirds of the operand traffic per SM) ran
-// at the tensor cores' 512 clocks a k-block without the additions, but with them was no faster: 265 to 288 us against 269 here, 160 to
-// 172 against 162 at 8192 x 7168 x 2048, 667 to 725 against 650 on 64 experts.  Sixteen accumulating warps instead of eight: 307 against 258.
+// What bounds it.  Many rows: a k-block of a 128 x 256 tile takes about 940 clocks, of which the tensor cores need 512 (8192 x 4096 x
+// 7168, clock64 around the 392 k-blocks of a CTA; from idle and back to back alike).  With the additions left out it takes 700, with
+// the loads from tensor memory left out as well 690: the operands come that slowly with nothing beside them, and the additions cost
+// the rest.  An accumulating warp by itself needs about 500.  The power cap makes every clock longer: 232 to 245 us from idle, 277
+// back to back at 985 W and 1.46 GHz (2.07 to 1.74 PFLOP/s); the library's product without block scales 178 and 198.  A form on CTA
+// pairs (cta_group::2, two thirds of the operand traffic per SM) ran at 512 clocks a k-block without the additions, but with them was
+// no faster: 265 to 288 us back to back where this one took 269, 160 to 172 against 162 at 8192 x 7168 x 2048, 667 to 725 against 650 on 64
+// experts.  Sixteen accumulating warps instead of eight: 307 against 258.
 // Few rows: reading the weights: 250 rows on 111 experts of 2048 x 4096 in 166 us, 5.6 TB/s.
 //
 // K need not be a multiple of 128: TMA fills what lies behind it with zeros.  Rows of a tile behind its group are computed
@@ -678,7 +681,7 @@ extern "C" int moe_fp8_gemm(const void* A, int64_t lda, const float* a_scale, in
     return launch<256, false, BM>(A, lda, B, p, tiles256, 1, dev.sm_count, st);
   int split = 1;
   while (split < MAX_SPLIT && p.k_blocks >= 4 * split && tiles128 * split * 2 <= (split == 1 ? dev.sm_count : dev.sm_count * 7 / 8)) split *= 2;
-  if (rows <= FEW_ROWS)      // nearly all of the ring holds weights then: a token through 4096 x 7168 11.8 -> 10.1 us
+  if (rows <= FEW_ROWS)      // nearly all of the ring holds weights then: a token through 4096 x 7168, weights in L2, 11.8 -> 10.1 us
     return split > 1 ? launch<128, true, FEW_ROWS>(A, lda, B, p, tiles128, split, dev.sm_count, st)
                      : launch<128, false, FEW_ROWS>(A, lda, B, p, tiles128, 1, dev.sm_count, st);
   return split > 1 ? launch<128, true, BM>(A, lda, B, p, tiles128, split, dev.sm_count, st)
