@@ -67,8 +67,8 @@ def _need_cuda(*ts: torch.Tensor) -> None:
 
 
 def _carried_out(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy where it is a conjugate or negative that its memory does not hold yet."""
-    return t.resolve_conj().resolve_neg() if t.is_neg() or t.is_conj() else t
+    """t, or a copy where it stands for the negative of what its memory holds."""
+    return t.resolve_neg() if t.is_neg() else t
 
 
 def status_buffer(device: torch.device) -> torch.Tensor:

@@ -205,6 +205,8 @@ def moe_permute(x: torch.Tensor, sort: MoESort) -> torch.Tensor:
         raise ValueError(f"x must be [{sort.tokens}, H], one row for each token of the sort")
     if x.device != sort.row_of.device:
         raise ValueError(f"x is on {x.device}, the sort's tables on {sort.row_of.device}")
+    if x.is_conj():
+        x = x.resolve_conj()
     backward = x.requires_grad and torch.is_grad_enabled()
     if backward and x.dtype not in _DTYPES:
         raise ValueError("the gradient of moe_permute is computed in bfloat16, float16 or float32")
